@@ -1,0 +1,368 @@
+// paged.cuh — what the operators over the paged cache share: the device-side view and
+// batch, the lookup of a token's place, the division of a ragged batch's attention over
+// the CTAs, TMA and mbarrier helpers, and the attention of one row from the definition.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "quant.cuh"
+
+#ifndef HDCE
+#define HDCE __host__ __device__ constexpr
+#endif
+
+namespace fiber {
+
+struct PagedView {
+    uint16_t *k, *v;  // 16-bit elements: fp16 or bf16
+    const int32_t *table;
+    int n_kv, page_shift, n_pages, n_slots, max_pages;
+    long long page_stride, head_stride, pos_stride;
+};
+
+struct RaggedDev {
+    int n_seqs, n_tokens;
+    int slot0;  // slot of sequence 0 when slot is null
+    const int32_t *q_start, *kv_len, *slot;
+};
+
+// A sequence as both operators read it: first token row, tokens, cached positions, slot.
+// A slot or length outside the table gives an empty cache (kv = 0).
+struct SeqInfo {
+    int q0, nq, kv, slot;
+};
+
+FDEV SeqInfo make_seq(const RaggedDev &b, const PagedView &kv, int start, int end, int len, int slot) {
+    SeqInfo s;
+    s.q0 = min(max(start, 0), b.n_tokens);
+    s.nq = min(max(end, s.q0), b.n_tokens) - s.q0;
+    const bool ok = slot >= 0 && slot < kv.n_slots && len >= 0 && len <= ((long long)kv.max_pages << kv.page_shift);
+    s.kv = ok ? len : 0;
+    s.slot = ok ? slot : 0;
+    return s;
+}
+
+// Position and slot of token `t`, by one warp; false when no sequence holds it. A 32-way
+// search over q_start down to 32 sequences, whose bounds, lengths and slots are then
+// loaded together.
+FDEV bool find_token(const RaggedDev &b, const PagedView &kv, int t, int lane, int &pos, int &slot) {
+    int lo = 0, n = b.n_seqs;
+    while (n > 32) {
+        const int step = (n + 31) / 32, i = lane * step;
+        const int v = i < n ? b.q_start[lo + i] : 0x7fffffff;
+        const int c = __popc(__ballot_sync(0xffffffffu, v <= t));
+        if (c == 0) return false;
+        lo += (c - 1) * step;
+        n = min(step, n - (c - 1) * step);
+    }
+    SeqInfo s = {0, 0, 0, 0};
+    if (lane < n)
+        s = make_seq(b, kv, b.q_start[lo + lane], b.q_start[lo + lane + 1], b.kv_len[lo + lane],
+                     b.slot ? b.slot[lo + lane] : b.slot0 + lo + lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, lane < n && t >= s.q0 && t < s.q0 + s.nq);
+    if (!hit) return false;
+    const int src = __ffs(hit) - 1;
+    pos = __shfl_sync(0xffffffffu, s.kv - s.nq - s.q0, src) + t;
+    slot = __shfl_sync(0xffffffffu, s.slot, src);
+    return true;
+}
+
+// ---- 16-bit types ------------------------------------------------------------------------
+
+template <bool BF>
+FDEV float2 unpack2(uint32_t w) {
+    if constexpr (BF)
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    else
+        return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <bool BF>
+FDEV uint32_t pack2(float a, float b) {  // a in the low half
+    uint32_t r;
+    if constexpr (BF)
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+// ---- mbarriers and TMA -------------------------------------------------------------------
+
+constexpr unsigned long long PG_WAIT_NS = 2000000000ull;
+
+FDEV uint32_t pg_saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+FDEV unsigned long long pg_now() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+FDEV void pg_init(uint64_t *bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(pg_saddr(bar)), "r"(count) : "memory");
+}
+FDEV bool pg_try(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(pg_saddr(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Waits for the phase of that parity; gives up when another thread of the CTA has
+// (*fail), or after PG_WAIT_NS (then sets *fail).
+static __device__ __noinline__ bool pg_wait_slow(uint64_t *bar, uint32_t parity, volatile int *fail) {
+    const unsigned long long t0 = pg_now();
+    for (;;) {
+        if (fail && *fail) return false;
+        for (int i = 0; i < 64; i++)
+            if (pg_try(bar, parity)) return true;
+        if (pg_now() - t0 > PG_WAIT_NS) {
+            if (fail) *fail = 1;
+            return false;
+        }
+    }
+}
+FDEV bool pg_wait(uint64_t *bar, uint32_t parity, volatile int *fail) {
+    return pg_try(bar, parity) || pg_wait_slow(bar, parity, fail);
+}
+FDEV void pg_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pg_saddr(bar)) : "memory");
+}
+FDEV void pg_expect_tx(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(pg_saddr(bar)), "r"(bytes) : "memory");
+}
+FDEV void pg_tma4(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(pg_saddr(bar))
+        : "memory");
+}
+FDEV void pg_tma3(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(pg_saddr(bar))
+        : "memory");
+}
+FDEV void pg_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- attention -----------------------------------------------------------------------------
+
+struct AttnPagedParams {
+    CUtensorMap kmap, vmap;  // (head_dim, page_size, n_kv, n_pages); 128-byte swizzle
+    CUtensorMap qmap;        // tile kernel: (head_dim, n_heads, n_tokens)
+    PagedView kv;
+    RaggedDev b;
+    const uint16_t *q;
+    uint16_t *out;
+    long long ldq, ldo;
+    int n_heads, group;  // group = n_heads / n_kv
+    int window;
+    float scale, scale_log2;  // scale * log2(e): scores in powers of two
+    int *status;              // workspace: set to 1 when a wait gave up
+    unsigned int *tickets;    // one per CTA, zero between calls
+    float *part_ml;           // [2 * n_cta][rows][2]: running maximum (powers of two) and sum
+    float *part_o;            // [2 * n_cta] unnormalised outputs
+};
+
+constexpr int PG_MAX_SEQS = 128;  // sequences of one launch; larger batches take several
+
+// How a launch's work is divided. The rows (token, head of the group) of a sequence and KV
+// head are cut into units of RU rows; a unit takes one step per tile of BK keys that any
+// of its rows sees (at least one, so rows that see nothing are written too). All steps in
+// the order (sequence, KV head, unit, tile) are numbered 0 .. T - 1 and CTA c of n takes
+// steps [c T / n, (c + 1) T / n): equal shares whatever the lengths. A unit that is
+// cut between CTAs leaves one softmax state per CTA; the last CTA to finish (ticket)
+// joins them in CTA order, so the result does not depend on the timing.
+struct AttnPlan {
+    uint32_t prefix[PG_MAX_SEQS + 1];
+    int4 seq[PG_MAX_SEQS];  // q0, nq, kv, slot
+};
+
+struct AttnUnit {
+    int s, g, i;           // sequence, KV head, unit of RU rows
+    int q0, nq, kv, slot;  // of the sequence
+    int row0, rows;        // rows of the unit: row0 .. row0 + rows - 1 of nq * group
+    int lo, hi;            // positions any row of the unit sees
+    uint32_t u0, steps;    // number of its first step, and its steps
+};
+
+// Positions that the rows [row0, row0 + rows) see together.
+FDEV void attn_span(int nq, int kv, int group, int window, int row0, int rows, int &lo, int &hi) {
+    const int p0 = kv - nq, t0 = row0 / group, t1 = (row0 + rows - 1) / group;
+    hi = max(0, p0 + t1 + 1);
+    lo = window > 0 ? max(0, p0 + t0 - window + 1) : 0;
+}
+
+FDEV uint32_t attn_steps(int nq, int kv, int group, int window, int ru, int bk_shift, int i) {
+    const int row0 = i * ru;
+    int lo, hi;
+    attn_span(nq, kv, group, window, row0, min(ru, nq * group - row0), lo, hi);
+    const int tiles = ((hi + (1 << bk_shift) - 1) >> bk_shift) - (lo >> bk_shift);
+    return (uint32_t)max(1, hi > lo ? tiles : 0);
+}
+
+// Fill the plan (all threads of the CTA; ends with a barrier) and return T.
+template <int THREADS>
+FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift) {
+    const int tid = threadIdx.x, lane = tid & 31, ns = p.b.n_seqs;
+    constexpr int SHORT = 8;  // sequences of more units are summed by whole warps
+    for (int s = tid; s < ns; s += THREADS) {
+        const SeqInfo q = make_seq(p.b, p.kv, p.b.q_start[s], p.b.q_start[s + 1], p.b.kv_len[s],
+                                   p.b.slot ? p.b.slot[s] : p.b.slot0 + s);
+        pl.seq[s] = make_int4(q.q0, q.nq, q.kv, q.slot);
+        const int nu = (q.nq * p.group + ru - 1) / ru;
+        uint32_t sum = 0;
+        if (nu <= SHORT)
+            for (int i = 0; i < nu; i++) sum += attn_steps(q.nq, q.kv, p.group, p.window, ru, bk_shift, i);
+        pl.prefix[s + 1] = sum;
+    }
+    if (tid == 0) pl.prefix[0] = 0;
+    __syncthreads();
+    for (int s = tid >> 5; s < ns; s += THREADS / 32) {
+        const int4 q = pl.seq[s];
+        const int nu = (q.y * p.group + ru - 1) / ru;
+        if (nu <= SHORT) continue;
+        uint32_t sum = 0;
+        for (int i = lane; i < nu; i += 32) sum += attn_steps(q.y, q.z, p.group, p.window, ru, bk_shift, i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) pl.prefix[s + 1] = sum;
+    }
+    __syncthreads();
+    if (tid < 32) {
+        uint32_t base = 0;
+        for (int s0 = 0; s0 < ns; s0 += 32) {
+            const int s = s0 + lane;
+            uint32_t v = s < ns ? pl.prefix[s + 1] * (uint32_t)p.kv.n_kv : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t t = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += t;
+            }
+            if (s < ns) pl.prefix[s + 1] = base + v;
+            base += __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    __syncthreads();
+    return pl.prefix[ns];
+}
+
+FDEV void attn_unit_fill(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift) {
+    const int4 q = pl.seq[u.s];
+    u.q0 = q.x;
+    u.nq = q.y;
+    u.kv = q.z;
+    u.slot = q.w;
+    u.row0 = u.i * ru;
+    u.rows = min(ru, u.nq * p.group - u.row0);
+    attn_span(u.nq, u.kv, p.group, p.window, u.row0, u.rows, u.lo, u.hi);
+    u.steps = attn_steps(u.nq, u.kv, p.group, p.window, ru, bk_shift, u.i);
+}
+
+// The unit that holds step x.
+FDEV void attn_unit_find(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift, uint32_t x) {
+    int a = 0, b = p.b.n_seqs;  // prefix[a] <= x < prefix[b]
+    while (b - a > 1) {
+        const int m = (a + b) >> 1;
+        if (pl.prefix[m] <= x)
+            a = m;
+        else
+            b = m;
+    }
+    u.s = a;
+    const uint32_t head = (pl.prefix[a + 1] - pl.prefix[a]) / (uint32_t)p.kv.n_kv;
+    uint32_t rem = x - pl.prefix[a];
+    u.g = (int)(rem / head);
+    rem -= (uint32_t)u.g * head;
+    const int4 q = pl.seq[a];
+    u.i = 0;
+    for (;;) {
+        const uint32_t n = attn_steps(q.y, q.z, p.group, p.window, ru, bk_shift, u.i);
+        if (rem < n) break;
+        rem -= n;
+        u.i++;
+    }
+    u.u0 = x - rem;
+    attn_unit_fill(u, pl, p, ru, bk_shift);
+}
+
+// The unit after u (the caller knows there is one).
+FDEV void attn_unit_next(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift) {
+    u.u0 += u.steps;
+    u.i++;
+    if (u.i * ru >= u.nq * p.group) {
+        u.i = 0;
+        u.g++;
+        if (u.g == p.kv.n_kv) {
+            u.g = 0;
+            do u.s++;
+            while (pl.prefix[u.s + 1] == pl.prefix[u.s]);  // sequences without tokens
+        }
+    }
+    attn_unit_fill(u, pl, p, ru, bk_shift);
+}
+
+// First step of CTA c's share, and the CTA that holds step x.
+FDEV uint32_t attn_share(uint32_t total, int n_cta, int c) { return (uint32_t)((unsigned long long)total * c / n_cta); }
+FDEV int attn_owner(uint32_t total, int n_cta, uint32_t x) {
+    return (int)((((unsigned long long)x + 1) * n_cta - 1) / total);
+}
+
+// One row from the definition, by one warp: only the positions the row sees are read, so
+// nothing behind a mask can reach it. Used for rows whose tile result is not finite: on
+// the tensor cores a masked position has weight 0, and 0 * inf or 0 * NaN is NaN.
+template <int HD, bool BF>
+static __device__ __noinline__ void attn_row_exact(const AttnPagedParams &p, const uint16_t *q, uint16_t *out, int slot,
+                                                   int g, int lo, int hi, int lane) {
+    const PagedView &c = p.kv;
+    const int mask = (1 << c.page_shift) - 1;
+    const int32_t *tab = c.table + (long long)slot * c.max_pages;
+    auto at = [&](int j) -> long long {  // -1: a table entry outside the pool reads as zeros
+        const int page = tab[j >> c.page_shift];
+        if (page < 0 || page >= c.n_pages) return -1;
+        return (long long)page * c.page_stride + (long long)g * c.head_stride + (long long)(j & mask) * c.pos_stride;
+    };
+    auto score = [&](int j) -> float {
+        const long long a = at(j);
+        if (a < 0) return 0.f;
+        float s = 0.f;
+        for (int d = 0; d < HD; d += 8) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(q + d), y = *reinterpret_cast<const uint4 *>(c.k + a + d);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 f = unpack2<BF>(xs[i]), h = unpack2<BF>(ys[i]);
+                s = fmaf(f.y, h.y, fmaf(f.x, h.x, s));
+            }
+        }
+        return s * p.scale;
+    };
+    float m = -INFINITY;
+    for (int j = lo + lane; j < hi; j += 32) m = fmaxf(m, score(j));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f, o2[HD / 32];
+#pragma unroll
+    for (int k = 0; k < HD / 32; k++) o2[k] = 0.f;
+    for (int j0 = lo; j0 < hi; j0 += 32) {
+        const float e = j0 + lane < hi ? expf(score(j0 + lane) - m) : 0.f;
+        l += e;
+        for (int i = 0; i < min(32, hi - j0); i++) {
+            const float w = __shfl_sync(0xffffffffu, e, i);
+            const long long a = at(j0 + i);
+#pragma unroll
+            for (int k = 0; k < HD / 32; k++) {
+                const uint32_t v = a < 0 ? 0u : c.v[a + lane + 32 * k];
+                o2[k] = fmaf(w, unpack2<BF>(v).x, o2[k]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+    for (int k = 0; k < HD / 32; k++) out[lane + 32 * k] = (uint16_t)pack2<BF>(o2[k] / l, 0.f);
+}
+
+}  // namespace fiber

@@ -240,3 +240,4 @@ def sample(logits: np.ndarray, temperature: float, top_k: int, top_p: float, sta
 
 
 from .cuda import *  # noqa: E402,F401,F403  (device API; loads lazily)
+from .paged import *  # noqa: E402,F401,F403  (operators over the paged cache)
