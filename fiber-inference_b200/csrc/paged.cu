@@ -14,6 +14,7 @@
 #include "launch.cuh"
 #include "paged_append.cuh"
 #include "paged_rows.cuh"
+#include "paged_tile.cuh"
 
 using namespace fiber;
 
@@ -139,6 +140,19 @@ bool pool_map(CUtensorMap *map, const void *pool, const fiber_kv_view_t *kv, int
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Map of the query rows: (head_dim, n_heads, n_tokens), box of 64 dims x the group's heads x
+// a tile's tokens.
+bool query_map(CUtensorMap *map, const void *q, int hd, int n_heads, int group, long long ldq, int n_tokens) {
+    auto enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n_heads, (cuuint64_t)n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)ldq * 2};
+    const cuuint32_t box[3] = {64u, (cuuint32_t)group, (cuuint32_t)(PT_ROWS / group)}, one[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(q), dims, strides, box, one,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <class TI, bool BF>
 cudaError_t launch_append(const AppendParams &p, int hd, cudaStream_t st) {
     const long long warps = (long long)p.b.n_tokens * append_warps_per_token(p.n_heads + 2 * p.kv.n_kv, hd);
@@ -153,28 +167,38 @@ constexpr size_t WS_TICKETS = 256, WS_PARTS = WS_TICKETS + 4096;
 constexpr int WS_MAX_CTAS = 1024;
 
 struct AttnShape {
-    int n_cta, rows;  // CTAs of a launch, rows of a unit
+    bool tile;        // tile kernel, else row kernel
+    int n_cta, rows;  // CTAs of a launch, rows of a unit's state
 };
 
 AttnShape attn_shape(const fiber_kv_view_t *kv, const fiber_ragged_t *b, int n_heads) {
-    (void)kv, (void)b, (void)n_heads;
-    return {std::min(sm_count() * PR_CTAS_PER_SM, WS_MAX_CTAS), PR_ROWS};
+    if (b->max_q * (long long)(n_heads / kv->n_kv_heads) > PR_ROWS)
+        return {true, std::min(sm_count(), WS_MAX_CTAS), 2 * PT_ROWS};
+    return {false, std::min(sm_count() * PR_CTAS_PER_SM, WS_MAX_CTAS), PR_ROWS};
 }
 
 size_t ws_bytes_of(const AttnShape &s, int hd) { return WS_PARTS + (size_t)2 * s.n_cta * s.rows * (hd + 2) * 4; }
 
-template <int HD, bool BF>
-cudaError_t launch_rows(const AttnPagedParams &p, int n_cta, cudaStream_t st) {
-    static bool ready[64];
+// Raise a kernel's shared-memory limit, once per device.
+template <class K>
+cudaError_t allow_smem(K kernel, int bytes, bool (&ready)[64]) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev >= 64 || !ready[dev]) {
-        e = cudaFuncSetAttribute(attn_rows_kernel<HD, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, pr_smem<HD>());
-        if (e != cudaSuccess) return e;
-        if (dev < 64) ready[dev] = true;
+    if (e != cudaSuccess || (dev < 64 && ready[dev])) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) ready[dev] = true;
+    return e;
+}
+
+template <int HD, bool BF>
+cudaError_t launch_attn(const AttnPagedParams &p, const AttnShape &s, cudaStream_t st) {
+    static bool ready_tile[64], ready_rows[64];
+    if (s.tile) {
+        cudaError_t e = allow_smem(attn_tile_kernel<HD, BF>, pt_smem<HD>(), ready_tile);
+        return e ? e : launch_pdl(attn_tile_kernel<HD, BF>, dim3(s.n_cta), dim3(PT_THREADS), pt_smem<HD>(), st, p);
     }
-    return launch_pdl(attn_rows_kernel<HD, BF>, dim3(n_cta), dim3(PR_THREADS), pr_smem<HD>(), st, p);
+    cudaError_t e = allow_smem(attn_rows_kernel<HD, BF>, pr_smem<HD>(), ready_rows);
+    return e ? e : launch_pdl(attn_rows_kernel<HD, BF>, dim3(s.n_cta), dim3(PR_THREADS), pr_smem<HD>(), st, p);
 }
 
 int check_attn(const char *fn, const fiber_kv_view_t *kv, const fiber_ragged_t *b, int n_heads) {
@@ -295,6 +319,7 @@ extern "C" int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t 
     p.ldo = ldo;
     p.n_heads = n_heads;
     p.group = n_heads / kv->n_kv_heads;
+    p.by_group = make_div((uint32_t)p.group);
     p.window = window;
     p.scale = scale;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
@@ -303,8 +328,10 @@ extern "C" int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t 
     p.tickets = (unsigned int *)(ws + WS_TICKETS);
     p.part_ml = (float *)(ws + WS_PARTS);
     p.part_o = p.part_ml + (size_t)2 * shape.n_cta * shape.rows * 2;
-    if (!pool_map(&p.kmap, kv->k_pool, kv, PR_BK) || !pool_map(&p.vmap, kv->v_pool, kv, PR_BK))
-        return fail(FIBER_ECUDA, "%s: cannot build the cache's tensor maps", fn);
+    const int bk = shape.tile ? PT_BK : PR_BK;
+    if (!pool_map(&p.kmap, kv->k_pool, kv, bk) || !pool_map(&p.vmap, kv->v_pool, kv, bk) ||
+        (shape.tile && !query_map(&p.qmap, d_q, hd, n_heads, p.group, ldq, batch->n_tokens)))
+        return fail(FIBER_ECUDA, "%s: cannot build the tensor maps", fn);
     cudaStream_t st = (cudaStream_t)stream;
     for (int s0 = 0; s0 < batch->n_seqs; s0 += PG_MAX_SEQS) {
         p.b.n_seqs = std::min(PG_MAX_SEQS, batch->n_seqs - s0);
@@ -314,9 +341,9 @@ extern "C" int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t 
         p.b.slot0 = s0;
         cudaError_t e;
         if (kv->type == FIBER_TYPE_F16)
-            e = hd == 64 ? launch_rows<64, false>(p, shape.n_cta, st) : launch_rows<128, false>(p, shape.n_cta, st);
+            e = hd == 64 ? launch_attn<64, false>(p, shape, st) : launch_attn<128, false>(p, shape, st);
         else
-            e = hd == 64 ? launch_rows<64, true>(p, shape.n_cta, st) : launch_rows<128, true>(p, shape.n_cta, st);
+            e = hd == 64 ? launch_attn<64, true>(p, shape, st) : launch_attn<128, true>(p, shape, st);
         if (e != cudaSuccess) return fail(FIBER_ECUDA, "%s: %s", fn, cudaGetErrorString(e));
     }
     return FIBER_OK;

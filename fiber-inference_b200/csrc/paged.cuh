@@ -13,6 +13,22 @@
 
 namespace fiber {
 
+// Division by a number known on the host: n / d = (mulhi(n, mul) + n) >> shift for n < 2^31.
+struct FastDiv {
+    uint32_t mul;
+    int shift;
+    uint32_t d;
+};
+inline FastDiv make_div(uint32_t d) {
+    FastDiv f;
+    f.shift = 0;
+    while ((1ull << f.shift) < d) f.shift++;
+    f.mul = (uint32_t)(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+    f.d = d;
+    return f;
+}
+FDEV int fdiv(int n, const FastDiv &f) { return (int)((__umulhi((uint32_t)n, f.mul) + (uint32_t)n) >> f.shift); }
+
 struct PagedView {
     uint16_t *k, *v;  // 16-bit elements: fp16 or bf16
     const int32_t *table;
@@ -110,7 +126,7 @@ FDEV bool pg_try(uint64_t *bar, uint32_t parity) {
 }
 // Waits for the phase of that parity; gives up when another thread of the CTA has
 // (*fail), or after PG_WAIT_NS (then sets *fail).
-static __device__ __noinline__ bool pg_wait_slow(uint64_t *bar, uint32_t parity, volatile int *fail) {
+static __device__ __forceinline__ bool pg_wait_slow(uint64_t *bar, uint32_t parity, volatile int *fail) {
     const unsigned long long t0 = pg_now();
     for (;;) {
         if (fail && *fail) return false;
@@ -158,6 +174,7 @@ struct AttnPagedParams {
     uint16_t *out;
     long long ldq, ldo;
     int n_heads, group;  // group = n_heads / n_kv
+    FastDiv by_group;
     int window;
     float scale, scale_log2;  // scale * log2(e): scores in powers of two
     int *status;              // workspace: set to 1 when a wait gave up
@@ -189,16 +206,16 @@ struct AttnUnit {
 };
 
 // Positions that the rows [row0, row0 + rows) see together.
-FDEV void attn_span(int nq, int kv, int group, int window, int row0, int rows, int &lo, int &hi) {
-    const int p0 = kv - nq, t0 = row0 / group, t1 = (row0 + rows - 1) / group;
+FDEV void attn_span(int nq, int kv, const AttnPagedParams &p, int row0, int rows, int &lo, int &hi) {
+    const int p0 = kv - nq, t0 = fdiv(row0, p.by_group), t1 = fdiv(row0 + rows - 1, p.by_group);
     hi = max(0, p0 + t1 + 1);
-    lo = window > 0 ? max(0, p0 + t0 - window + 1) : 0;
+    lo = p.window > 0 ? max(0, p0 + t0 - p.window + 1) : 0;
 }
 
-FDEV uint32_t attn_steps(int nq, int kv, int group, int window, int ru, int bk_shift, int i) {
+FDEV uint32_t attn_steps(int nq, int kv, const AttnPagedParams &p, int ru, int bk_shift, int i) {
     const int row0 = i * ru;
     int lo, hi;
-    attn_span(nq, kv, group, window, row0, min(ru, nq * group - row0), lo, hi);
+    attn_span(nq, kv, p, row0, min(ru, nq * p.group - row0), lo, hi);
     const int tiles = ((hi + (1 << bk_shift) - 1) >> bk_shift) - (lo >> bk_shift);
     return (uint32_t)max(1, hi > lo ? tiles : 0);
 }
@@ -215,7 +232,7 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
         const int nu = (q.nq * p.group + ru - 1) / ru;
         uint32_t sum = 0;
         if (nu <= SHORT)
-            for (int i = 0; i < nu; i++) sum += attn_steps(q.nq, q.kv, p.group, p.window, ru, bk_shift, i);
+            for (int i = 0; i < nu; i++) sum += attn_steps(q.nq, q.kv, p, ru, bk_shift, i);
         pl.prefix[s + 1] = sum;
     }
     if (tid == 0) pl.prefix[0] = 0;
@@ -225,7 +242,7 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
         const int nu = (q.y * p.group + ru - 1) / ru;
         if (nu <= SHORT) continue;
         uint32_t sum = 0;
-        for (int i = lane; i < nu; i += 32) sum += attn_steps(q.y, q.z, p.group, p.window, ru, bk_shift, i);
+        for (int i = lane; i < nu; i += 32) sum += attn_steps(q.y, q.z, p, ru, bk_shift, i);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) pl.prefix[s + 1] = sum;
@@ -257,8 +274,8 @@ FDEV void attn_unit_fill(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
     u.slot = q.w;
     u.row0 = u.i * ru;
     u.rows = min(ru, u.nq * p.group - u.row0);
-    attn_span(u.nq, u.kv, p.group, p.window, u.row0, u.rows, u.lo, u.hi);
-    u.steps = attn_steps(u.nq, u.kv, p.group, p.window, ru, bk_shift, u.i);
+    attn_span(u.nq, u.kv, p, u.row0, u.rows, u.lo, u.hi);
+    u.steps = attn_steps(u.nq, u.kv, p, ru, bk_shift, u.i);
 }
 
 // The unit that holds step x.
@@ -279,7 +296,7 @@ FDEV void attn_unit_find(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
     const int4 q = pl.seq[a];
     u.i = 0;
     for (;;) {
-        const uint32_t n = attn_steps(q.y, q.z, p.group, p.window, ru, bk_shift, u.i);
+        const uint32_t n = attn_steps(q.y, q.z, p, ru, bk_shift, u.i);
         if (rem < n) break;
         rem -= n;
         u.i++;

@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         int rlo[2], rhi[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int r = g8 + 8 * h, t = (u.row0 + r) / p.group, head = u.g * p.group + (u.row0 + r) % p.group;
+            const int r = g8 + 8 * h, t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
             const bool in = r < u.rows;
             rhi[h] = in ? p0 + t + 1 : 0;
             rlo[h] = p.window > 0 ? max(0, p0 + t - p.window + 1) : 0;
@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
 #pragma unroll
         for (int n = 0; n < HD / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
         // every row of the unit sees the keys in [all_lo, all_hi): no mask needed there
-        const int all_hi = max(0, p0 + u.row0 / p.group + 1);
-        const int all_lo = p.window > 0 ? max(0, p0 + (u.row0 + u.rows - 1) / p.group - p.window + 1) : 0;
+        const int all_hi = max(0, p0 + fdiv(u.row0, p.by_group) + 1);
+        const int all_lo = p.window > 0 ? max(0, p0 + fdiv(u.row0 + u.rows - 1, p.by_group) - p.window + 1) : 0;
         int st = 0;
         if (any) {
             for (uint32_t k = b; k < e; k++, it++) {
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                 }
                 if (whole) {
                     const float inv = 1.f / L;
-                    const int t = (u.row0 + r) / p.group, head = u.g * p.group + (u.row0 + r) % p.group;
+                    const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
                     const bool sees = p0 + t >= 0;
                     a = sees ? make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
                     if (!(isfinite(a.x) && isfinite(a.y) && isfinite(a.z) && isfinite(a.w))) atomicOr(&sh.bad, 1u << r);
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                             a.z = fmaf(f, v.z, a.z);
                             a.w = fmaf(f, v.w, a.w);
                         }
-                        const int t = (u.row0 + r) / p.group, head = u.g * p.group + (u.row0 + r) % p.group;
+                        const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
                         const bool sees = p0 + t >= 0;
                         a = sees ? make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
                         if (!(isfinite(a.x) && isfinite(a.y) && isfinite(a.z) && isfinite(a.w))) atomicOr(&sh.bad, 1u << r);
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
             if (bad) {
                 for (int r = warp; r < u.rows; r += PR_WARPS) {
                     if (!(bad >> r & 1)) continue;
-                    const int t = (u.row0 + r) / p.group, head = u.g * p.group + (u.row0 + r) % p.group;
+                    const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
                     attn_row_exact<HD, BF>(p, p.q + (long long)(u.q0 + t) * p.ldq + (long long)head * HD,
                                            p.out + (long long)(u.q0 + t) * p.ldo + (long long)head * HD, u.slot, u.g,
                                            p.window > 0 ? max(0, p0 + t - p.window + 1) : 0, p0 + t + 1, lane);
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         } else {
             for (int i = tid; i < u.rows * C4; i += 32 * PR_WARPS) {
                 const int r = i / C4, c4 = i % C4;
-                const int t = (u.row0 + r) / p.group, head = u.g * p.group + (u.row0 + r) % p.group;
+                const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
                 *reinterpret_cast<uint2 *>(p.out + (long long)(u.q0 + t) * p.ldo + (long long)head * HD + 4 * c4) =
                     make_uint2(0u, 0u);
             }

@@ -1,0 +1,565 @@
+// paged_tile.cuh — attention over the paged cache for chunks of tokens on the
+// 5th-generation tensor cores.
+//
+// A unit is two tiles (A, B) of up to 128 rows (token, head of the group) of one sequence
+// and KV head, and walks the 128-key tiles that its rows see. One CTA per SM:
+//   warps 0-3   softmax of tile A, one row per thread: scores from tensor memory, running
+//               maximum and sum, probabilities back to tensor memory in 16 bits
+//   warps 4-7   the same for tile B
+//   warp 8      one lane issues the MMAs: S = Q K^T (operands in shared memory), then
+//               O += P V with P read from tensor memory
+//   warp 9      producer: Q, K and V tiles by TMA (K / V boxes go page by page)
+// Tensor memory: S_A, S_B (128 columns each; P overwrites the front half of its S), O_A,
+// O_B (head_dim columns each). While one tile's softmax runs, the tensor core works on
+// the other's products.
+//
+// The output accumulators are rescaled only when a row's maximum has grown by more than
+// 2^8 since the last time (the probabilities, at most 2^8, keep their 11 or 8 bits); the
+// softmax warps do it themselves, since S of the next tile is only reported after the
+// product that last wrote O.
+#pragma once
+#include "paged.cuh"
+
+namespace fiber {
+
+constexpr int PT_ROWS = 128;                          // rows of a tile
+constexpr int PT_BK_SHIFT = 7, PT_BK = 1 << PT_BK_SHIFT;  // keys of a tile
+constexpr int PT_THREADS = 384;  // three warpgroups; warps 10 and 11 only make up the third
+constexpr float PT_GROWTH = 8.f;  // powers of two a row's maximum may grow before O is rescaled
+
+// Tokens and rows of a tile: whole tokens (all heads of the group).
+HDCE int pt_tile_rows(int group) { return PT_ROWS / group * group; }
+
+template <int HD>
+HDCE int pt_tile_bytes() { return 128 * HD * 2; }  // a Q, K or V tile: [HD / 64][128 rows][128 B], 128-byte swizzle
+template <int HD>
+HDCE int pt_stages() { return HD == 128 ? 5 : 8; }
+
+struct PtShared {
+    AttnPlan plan;
+    uint64_t kvfull[8], kvfree[8];
+    uint64_t qfull, qfree;
+    uint64_t sfull[2], pready[2], odone[2];
+    uint64_t mdone;
+    uint32_t tmem;
+    int last;
+    int fail;
+};
+template <int HD>
+HDCE int pt_smem() { return (2 + pt_stages<HD>()) * pt_tile_bytes<HD>() + (int)sizeof(PtShared); }
+
+FDEV uint64_t pt_desc(uint32_t saddr, uint32_t lbo) {
+    // 128-byte swizzle (2 << 61), version 1, 8-row groups 1024 B apart; lbo: for the operand
+    // whose rows are K (V), the next 64 columns
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// kind::f16: D fp32, A and B both fp16 or both bf16, M 128; b_rows_k: B is [K][N] in memory
+template <bool BF>
+HDCE uint32_t pt_idesc(int n, bool b_rows_k) {
+    return (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((b_rows_k ? 1u : 0u) << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// The issuing warp runs converged and every MMA and commit is predicated on its elected
+// lane: descriptors then stay in uniform registers. Issued from a divergent branch
+// (lane 0 alone) each operand is moved there one by one, about 130 cycles per MMA of 64.
+FDEV uint32_t pt_elect() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
+}
+FDEV void pt_mma_ss(uint32_t me, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(me)
+        : "memory");
+}
+FDEV void pt_mma_ts(uint32_t me, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(me)
+        : "memory");
+}
+FDEV void pt_commit(uint32_t me, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(pg_saddr(bar)),
+        "r"(me)
+        : "memory");
+}
+FDEV void pt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+FDEV void pt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+FDEV void pt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+FDEV void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes (one row per thread)
+FDEV void pt_ld32(float *v, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+          "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(addr)
+        : "memory");
+}
+FDEV void pt_ld16(float *v, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(addr)
+        : "memory");
+}
+FDEV void pt_st16(uint32_t addr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+FDEV float pt_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The lowest n bits (none below 0, all from 32)
+FDEV uint32_t pt_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
+FDEV void pt_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// A unit's piece [b, e) of steps, as every warp of the CTA sees it.
+struct PtPiece {
+    uint32_t b, e;
+    int kt0;       // key tile of step 0
+    int rows[2];   // rows of tile A, B
+    int ab[2], ae[2];  // steps [ab, ae) in which the tile has work
+};
+FDEV void pt_piece(PtPiece &q, const AttnUnit &u, const AttnPagedParams &p, int rt, uint32_t x, uint32_t x1) {
+    q.b = x - u.u0;
+    q.e = min(x1 - u.u0, u.steps);
+    q.kt0 = u.lo >> PT_BK_SHIFT;
+    const bool any = u.hi > u.lo;
+    q.rows[0] = min(rt, u.rows);
+    q.rows[1] = u.rows - q.rows[0];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        int lo = 0, hi = 0;
+        if (q.rows[t] > 0 && any) attn_span(u.nq, u.kv, p, u.row0 + t * rt, q.rows[t], lo, hi);
+        if (hi > lo) {
+            q.ab[t] = max((int)q.b, (lo >> PT_BK_SHIFT) - q.kt0);
+            q.ae[t] = min((int)q.e, ((hi + PT_BK - 1) >> PT_BK_SHIFT) - q.kt0);
+        } else {
+            q.ab[t] = q.ae[t] = 0;
+        }
+        if (q.ae[t] < q.ab[t]) q.ae[t] = q.ab[t];
+    }
+}
+FDEV bool pt_on(const PtPiece &q, int t, int k) { return k >= q.ab[t] && k < q.ae[t]; }
+
+template <int HD, bool BF>
+__global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_constant__ AttnPagedParams p) {
+    constexpr int NST = pt_stages<HD>(), TB = pt_tile_bytes<HD>(), HALVES = HD / 64;
+    extern __shared__ __align__(1024) uint8_t pt_raw[];
+    uint8_t *qbuf = pt_raw, *ring = pt_raw + 2 * TB;
+    PtShared &sh = *reinterpret_cast<PtShared *>(ring + NST * TB);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (pg_saddr(pt_raw) & 1023u) {  // never: the operand tiles must start on 1024 bytes
+        if (tid == 0) *p.status = 2;
+        return;
+    }
+    if (tid == 0) {
+        for (int s = 0; s < NST; s++) {
+            pg_init(&sh.kvfull[s], 1);
+            pg_init(&sh.kvfree[s], 1);
+        }
+        pg_init(&sh.qfull, 1);
+        pg_init(&sh.qfree, 1);
+        for (int t = 0; t < 2; t++) {
+            pg_init(&sh.sfull[t], 1);
+            pg_init(&sh.pready[t], 4);
+            pg_init(&sh.odone[t], 1);
+        }
+        pg_init(&sh.mdone, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        sh.fail = 0;
+    }
+    pdl_trigger();
+    pdl_wait();
+    const int rt = pt_tile_rows(p.group), ru = 2 * rt;
+    const uint32_t total = attn_plan_build<PT_THREADS>(sh.plan, p, ru, PT_BK_SHIFT);
+    const int n_cta = min((int)gridDim.x, (int)min(total, 0x7fffffffu)), cta = blockIdx.x;
+    if (cta >= n_cta) return;
+    const uint32_t x0 = attn_share(total, n_cta, cta), x1 = attn_share(total, n_cta, cta + 1);
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pg_saddr(&sh.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pt_fence_before();
+    __syncthreads();
+    pt_fence_after();
+    if (sh.tmem != 0 && tid == 0) *p.status = 2;  // never: all 512 columns start at column 0
+    constexpr uint32_t tmem = 0;
+    AttnUnit u;
+    attn_unit_find(u, sh.plan, p, ru, PT_BK_SHIFT, x0);
+    PtPiece q;
+    // 384 threads at 168 registers: the softmax warpgroups take 224 each, the third keeps 56
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 9) {
+            // ---- producer: lane b issues box b of a K or V tile
+            const int box_rows = min(1 << p.kv.page_shift, PT_BK), nrb = PT_BK / box_rows;
+            const int half = lane / nrb, rb = lane % nrb, mask = (1 << p.kv.page_shift) - 1;
+            const bool boxed = lane < HALVES * nrb;
+            const uint32_t dst0 = half * (128 * 128) + rb * box_rows * 128;
+            uint32_t it = 0, nq = 0;  // K / V tiles and Q pairs issued
+            bool ok = true;
+            for (uint32_t x = x0;;) {
+                pt_piece(q, u, p, rt, x, x1);
+                if (q.ae[0] > q.ab[0] || q.ae[1] > q.ab[1]) {
+                    const int32_t *tab = p.kv.table + (long long)u.slot * p.kv.max_pages;
+                    const int used = (u.hi + mask) >> p.kv.page_shift;
+                    for (uint32_t k = q.b; k < q.e; k++) {
+                        const int key = ((q.kt0 + (int)k) << PT_BK_SHIFT) + rb * box_rows, lp = key >> p.kv.page_shift;
+                        int page = p.kv.n_pages;  // outside the tensor: reads as zeros
+                        if (boxed && lp < used) page = tab[lp];
+    #pragma unroll
+                        for (int v = 0; v < 2; v++, it++) {
+                            const int st = it % NST;
+                            if (it >= NST) ok = pg_wait(&sh.kvfree[st], (it / NST - 1) & 1, &sh.fail);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            if (lane == 0) pg_expect_tx(&sh.kvfull[st], TB);
+                            __syncwarp();
+                            if (boxed)
+                                pg_tma4(pg_saddr(ring + st * TB) + dst0, v ? &p.vmap : &p.kmap, half * 64, key & mask, u.g, page,
+                                        &sh.kvfull[st]);
+                        }
+                        if (!ok) break;
+                        if (k == q.b) {  // the queries' buffer is free last: K and V of the first step go before
+                            if (nq > 0) ok = pg_wait(&sh.qfree, (nq - 1) & 1, &sh.fail);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            if (lane == 0) {
+                                const int nt = q.rows[1] > 0 ? 2 : 1;
+                                pg_expect_tx(&sh.qfull, (uint32_t)(nt * HALVES * rt * 128));
+                                for (int t = 0; t < nt; t++)
+                                    for (int h = 0; h < HALVES; h++)
+                                        pg_tma3(pg_saddr(qbuf + t * TB) + h * (128 * 128), &p.qmap, 64 * h, u.g * p.group,
+                                                u.q0 + fdiv(u.row0 + t * rt, p.by_group), &sh.qfull);
+                            }
+                            nq++;
+                        }
+                    }
+                }
+                x = u.u0 + q.e;
+                if (!ok || x >= x1) break;
+                attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+            }
+            if (lane == 0) {  // every copy has landed before the CTA exits
+                for (uint32_t s = 0; s < NST && s < it; s++)
+                    pg_wait(&sh.kvfull[s], (s + (it - 1 - s) / NST * NST) / NST & 1, nullptr);
+                if (nq > 0) pg_wait(&sh.qfull, (nq - 1) & 1, nullptr);
+            }
+        } else if (warp == 8) {
+            // ---- MMA issuer
+            constexpr uint32_t IS = pt_idesc<BF>(PT_BK, false), IO = pt_idesc<BF>(HD, true);
+            const uint32_t me = pt_elect();
+            uint32_t nq = 0, np[2] = {0, 0};
+            int ks = 0, kph = 0;  // ring stage and parity of step k's K tile; its V tile is the next
+            bool ok = true;
+            auto after = [&](int &st, int &ph, int n) {
+                st += n;
+                if (st >= NST) {
+                    st -= NST;
+                    ph ^= 1;
+                }
+            };
+            auto scores = [&](int t, int st) {  // S_t = Q_t K^T
+                const uint64_t a = pt_desc(pg_saddr(qbuf) + t * TB, 16), b = pt_desc(pg_saddr(ring) + st * TB, 16);
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++) {
+                    const uint32_t o = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                    pt_mma_ss(me, t * 128, a + o, b + o, IS, k > 0);
+                }
+                pt_commit(me, &sh.sfull[t]);
+            };
+            auto values = [&](int t, int st, bool first) {  // O_t += P_t V
+                const uint64_t b = pt_desc(pg_saddr(ring) + st * TB, 128 * 128);
+#pragma unroll
+                for (int k = 0; k < PT_BK / 16; k++)
+                    pt_mma_ts(me, 256 + t * 128, t * 128 + 8 * k, b + k * (2048 >> 4), IO, !first || k > 0);
+            };
+            for (uint32_t x = x0; ok;) {
+                pt_piece(q, u, p, rt, x, x1);
+                if (q.ae[0] > q.ab[0] || q.ae[1] > q.ab[1]) {
+                    ok = pg_wait(&sh.qfull, nq & 1, &sh.fail) && pg_wait(&sh.kvfull[ks], kph, &sh.fail);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    nq++;
+                    pt_fence_after();
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+                        if (pt_on(q, t, q.b)) scores(t, ks);
+                    pt_commit(me, &sh.kvfree[ks]);
+                    if (q.e - q.b == 1) pt_commit(me, &sh.qfree);
+                    for (int k = q.b; k < (int)q.e; k++) {
+                        const bool more = k + 1 < (int)q.e;
+                        int vs = ks, vph = kph;
+                        after(vs, vph, 1);
+                        int ns = vs, nph = vph;  // the next step's K tile
+                        after(ns, nph, 1);
+                        if (more) ok = pg_wait(&sh.kvfull[ns], nph, &sh.fail);
+                        ok = ok && pg_wait(&sh.kvfull[vs], vph, &sh.fail);
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            if (pt_on(q, t, k)) {
+                                ok = ok && pg_wait(&sh.pready[t], np[t] & 1, &sh.fail);
+                                ok = __all_sync(0xffffffffu, ok);
+                                if (!ok) break;
+                                np[t]++;
+                                pt_fence_after();
+                                values(t, vs, k == q.ab[t]);
+                                if (k + 1 == q.ae[t]) pt_commit(me, &sh.odone[t]);
+                            }
+                            if (t == 1) pt_commit(me, &sh.kvfree[vs]);
+                            if (more && pt_on(q, t, k + 1)) scores(t, ns);
+                        }
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (more) pt_commit(me, &sh.kvfree[ns]);
+                        if (k + 2 == (int)q.e) pt_commit(me, &sh.qfree);
+                        ks = ns;
+                        kph = nph;
+                    }
+                }
+                x = u.u0 + q.e;
+                if (x >= x1) break;
+                attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+            }
+            pt_commit(me, &sh.mdone);  // every product has finished before tensor memory is released
+            pg_wait(&sh.mdone, 0, nullptr);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ---- softmax: thread = row of tile t
+        const int t = warp >> 2, row = tid & 127;
+        const uint32_t sa = tmem + t * 128 + ((uint32_t)(32 * (warp & 3)) << 16), oa = sa + 256;
+        uint32_t it = 0, ns = 0, no = 0;
+        for (uint32_t x = x0;;) {
+            pt_piece(q, u, p, rt, x, x1);
+            const bool whole = q.b == 0 && q.e == u.steps;
+            const bool run = q.ae[0] > q.ab[0] || q.ae[1] > q.ab[1];
+            const int p0 = u.kv - u.nq, tok = fdiv(u.row0 + t * rt + row, p.by_group), head = u.g * p.group + u.row0 + t * rt + row - tok * p.group;
+            const bool in = row < q.rows[t];
+            const int rhi = in ? p0 + tok + 1 : 0, rlo = p.window > 0 ? max(0, p0 + tok - p.window + 1) : 0;
+            // every row of the tile sees the keys in [all_lo, all_hi)
+            const int all_hi = q.rows[t] > 0 ? p0 + fdiv(u.row0 + t * rt, p.by_group) + 1 : 0;
+            const int all_lo = p.window > 0 && q.rows[t] > 0 ? max(0, p0 + fdiv(u.row0 + t * rt + q.rows[t] - 1, p.by_group) - p.window + 1) : 0;
+            float m = -INFINITY, l = 0.f;
+            if (run) {
+                for (int k = q.b; k < (int)q.e; k++, it += 2) {
+                    if (!pt_on(q, t, k)) continue;
+                    const int key0 = (q.kt0 + k) << PT_BK_SHIFT;
+                    pg_wait(&sh.sfull[t], ns & 1, &sh.fail);  // after a timeout: runs through, status says so
+                    ns++;
+                    pt_fence_after();
+                    float s[128];
+#pragma unroll
+                    for (int c = 0; c < 128; c += 32) pt_ld32(s + c, sa + c);
+                    pt_wait_ld();
+                    if (key0 < all_lo || key0 + PT_BK > all_hi) {
+                        const int a = rlo - key0, b = rhi - key0;  // columns [a, b) are seen
+#pragma unroll
+                        for (int c = 0; c < 128; c += 32) {
+                            const uint32_t keep = pt_below(b - c) & ~pt_below(a - c);
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (!(keep >> j & 1)) s[c + j] = -INFINITY;
+                        }
+                    }
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                    const bool grow = mt > m + PT_GROWTH || (m == -INFINITY && mt > m);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float mn = grow ? mt : m;
+                        const float f = grow ? pt_exp2(m - mn) : 1.f;
+                        m = mn;
+                        l *= f;
+                        if (k > q.ab[t]) {
+#pragma unroll
+                            for (int c = 0; c < HD; c += 16) {
+                                float o[16];
+                                uint32_t w[16];
+                                pt_ld16(o, oa + c);
+                                pt_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 16; j++) w[j] = __float_as_uint(o[j] * f);
+                                pt_st16(oa + c, w);
+                            }
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 128; c += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const float a = pt_exp2(fmaf(s[c + 2 * j], p.scale_log2, -base));
+                            const float b = pt_exp2(fmaf(s[c + 2 * j + 1], p.scale_log2, -base));
+                            sum[(2 * j) & 3] += a;
+                            sum[(2 * j + 1) & 3] += b;
+                            w[j] = pack2<BF>(a, b);
+                        }
+                        pt_st16(sa + c / 2, w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    if ((key0 < u.lo || key0 + PT_BK > u.hi) && (t == 0 || !pt_on(q, 0, k))) {
+                        // values no row of the unit sees may hold anything: weight 0 must meet 0 there
+                        const uint32_t vi = it + 1;
+                        pg_wait(&sh.kvfull[vi % NST], vi / NST & 1, &sh.fail);
+                        if (key0 + row < u.lo || key0 + row >= u.hi)
+#pragma unroll 1
+                            for (int c = 0; c < 8 * HALVES; c++)  // pieces rotated by the row: eight rows on eight banks
+                                *reinterpret_cast<uint4 *>(ring + (vi % NST) * TB + (c >> 3) * (128 * 128) + row * 128 +
+                                                           (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                        pg_proxy_fence();
+                    }
+                    pt_wait_st();
+                    pt_fence_before();
+                    __syncwarp();
+                    if (lane == 0) pg_arrive(&sh.pready[t]);
+                }
+            }
+            // ---- the unit's (or piece's) output
+            const bool did = q.ae[t] > q.ab[t];
+            if (did) {
+                pg_wait(&sh.odone[t], no & 1, &sh.fail);
+                no++;
+                pt_fence_after();
+            }
+            uint16_t *dst = p.out + (long long)(u.q0 + tok) * p.ldo + (long long)head * HD;
+            bool bad = false;
+            auto store32 = [&](int c, const float *o) {  // 32 output values of this thread's row
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) bad |= !isfinite(o[j + i]);
+                    *reinterpret_cast<uint4 *>(dst + c + j) =
+                        make_uint4(pack2<BF>(o[j], o[j + 1]), pack2<BF>(o[j + 2], o[j + 3]), pack2<BF>(o[j + 4], o[j + 5]),
+                                   pack2<BF>(o[j + 6], o[j + 7]));
+                }
+            };
+            if (whole) {
+                const float inv = 1.f / l;
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    float o[32];
+                    if (did) {
+                        pt_ld32(o, oa + c);
+                        pt_wait_ld();
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j++) o[j] = did && rhi > rlo ? o[j] * inv : 0.f;
+                    if (in) store32(c, o);
+                }
+            } else {
+                const int pslot = 2 * cta + (q.b > 0 ? 0 : 1);
+                float4 *po = reinterpret_cast<float4 *>(p.part_o) + (long long)(2 * pslot + t) * (HD / 4) * 128 + row;
+                float *pm = p.part_ml + (2 * pslot + t) * 256 + row;
+                if (q.rows[t] > 0) {
+                    pm[0] = did ? m : -INFINITY;
+                    pm[128] = l;
+                    if (did)
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32) {
+                            float o[32];
+                            pt_ld32(o, oa + c);
+                            pt_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) po[(c + j) / 4 * 128] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        }
+                }
+                const int ca = attn_owner(total, n_cta, u.u0), cb = attn_owner(total, n_cta, u.u0 + u.steps - 1);
+                __threadfence();
+                pt_bar();
+                if (tid == 0) {
+                    sh.last = atomicAdd(&p.tickets[ca], 1u) == (unsigned)(cb - ca);
+                    if (sh.last) p.tickets[ca] = 0u;
+                    __threadfence();
+                }
+                pt_bar();
+                if (sh.last && q.rows[t] > 0) {
+                    float M = -INFINITY, L = 0.f;
+                    for (int c = ca; c <= cb; c++)
+                        M = fmaxf(M, __ldcg(p.part_ml + (2 * (2 * c + (c == ca)) + t) * 256 + row));
+                    for (int c = ca; c <= cb; c++) {
+                        const float *ml = p.part_ml + (2 * (2 * c + (c == ca)) + t) * 256 + row;
+                        const float mc = __ldcg(ml);
+                        if (mc != -INFINITY) L = fmaf(pt_exp2(mc - M), __ldcg(ml + 128), L);
+                    }
+                    const float inv = rhi > rlo ? 1.f / L : 0.f;
+                    float o[HD];
+#pragma unroll
+                    for (int j = 0; j < HD; j++) o[j] = 0.f;
+#pragma unroll 1
+                    for (int c = ca; c <= cb; c++) {
+                        const int sl = 2 * (2 * c + (c == ca)) + t;
+                        const float mc = __ldcg(p.part_ml + sl * 256 + row);
+                        const float4 *src = reinterpret_cast<const float4 *>(p.part_o) + (long long)sl * (HD / 4) * 128 + row;
+                        const float f = pt_exp2(mc - M);
+#pragma unroll
+                        for (int j0 = 0; j0 < HD / 4; j0 += 16) {
+                            float4 v[16];
+#pragma unroll
+                            for (int j = 0; j < 16; j++) v[j] = __ldcg(src + (j0 + j) * 128);
+                            if (mc != -INFINITY)  // else no key of its part seen
+#pragma unroll
+                                for (int j = 0; j < 16; j++) {
+                                    float *a = o + 4 * (j0 + j);
+                                    a[0] = fmaf(f, v[j].x, a[0]);
+                                    a[1] = fmaf(f, v[j].y, a[1]);
+                                    a[2] = fmaf(f, v[j].z, a[2]);
+                                    a[3] = fmaf(f, v[j].w, a[3]);
+                                }
+                        }
+                    }
+                    if (in)
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++) o[c + j] = rhi > rlo ? o[c + j] * inv : 0.f;
+                            store32(c, o + c);
+                        }
+                }
+            }
+            // rows whose result is not finite, again and exactly
+            unsigned again = __ballot_sync(0xffffffffu, bad);
+            while (again) {
+                const int src = __ffs(again) - 1;
+                again &= again - 1;
+                const int stok = __shfl_sync(0xffffffffu, tok, src), shead = __shfl_sync(0xffffffffu, head, src);
+                attn_row_exact<HD, BF>(p, p.q + (long long)(u.q0 + stok) * p.ldq + (long long)shead * HD,
+                                       p.out + (long long)(u.q0 + stok) * p.ldo + (long long)shead * HD, u.slot, u.g,
+                                       __shfl_sync(0xffffffffu, rlo, src), __shfl_sync(0xffffffffu, rhi, src), lane);
+            }
+            x = u.u0 + q.e;
+            if (x >= x1) break;
+            attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+        }
+    }
+    pt_fence_before();
+    __syncthreads();
+    if (tid == 0 && sh.fail) *p.status = 1;
+    if (warp == 8) {
+        pt_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+}  // namespace fiber
