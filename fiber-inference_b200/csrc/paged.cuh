@@ -174,7 +174,7 @@ struct AttnPagedParams {
     uint16_t *out;
     long long ldq, ldo;
     int n_heads, group;  // group = n_heads / n_kv
-    FastDiv by_group;
+    FastDiv by_group, by_ru;  // by_ru: rows of a unit
     int window;
     float scale, scale_log2;  // scale * log2(e): scores in powers of two
     int *status;              // workspace: set to 1 when a wait gave up
@@ -229,7 +229,7 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
         const SeqInfo q = make_seq(p.b, p.kv, p.b.q_start[s], p.b.q_start[s + 1], p.b.kv_len[s],
                                    p.b.slot ? p.b.slot[s] : p.b.slot0 + s);
         pl.seq[s] = make_int4(q.q0, q.nq, q.kv, q.slot);
-        const int nu = (q.nq * p.group + ru - 1) / ru;
+        const int nu = fdiv(q.nq * p.group + ru - 1, p.by_ru);
         uint32_t sum = 0;
         if (nu <= SHORT)
             for (int i = 0; i < nu; i++) sum += attn_steps(q.nq, q.kv, p, ru, bk_shift, i);
@@ -239,7 +239,7 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
     __syncthreads();
     for (int s = tid >> 5; s < ns; s += THREADS / 32) {
         const int4 q = pl.seq[s];
-        const int nu = (q.y * p.group + ru - 1) / ru;
+        const int nu = fdiv(q.y * p.group + ru - 1, p.by_ru);
         if (nu <= SHORT) continue;
         uint32_t sum = 0;
         for (int i = lane; i < nu; i += 32) sum += attn_steps(q.y, q.z, p, ru, bk_shift, i);
@@ -278,15 +278,15 @@ FDEV void attn_unit_fill(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
     u.steps = attn_steps(u.nq, u.kv, p, ru, bk_shift, u.i);
 }
 
-// The unit that holds step x.
+// The unit that holds step x; all lanes of a warp together.
 FDEV void attn_unit_find(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift, uint32_t x) {
+    const int lane = threadIdx.x & 31;
     int a = 0, b = p.b.n_seqs;  // prefix[a] <= x < prefix[b]
     while (b - a > 1) {
-        const int m = (a + b) >> 1;
-        if (pl.prefix[m] <= x)
-            a = m;
-        else
-            b = m;
+        const int step = (b - a + 31) / 32, i = a + lane * step;
+        const int c = __popc(__ballot_sync(0xffffffffu, i < b && pl.prefix[min(i, b)] <= x));
+        a += (c - 1) * step;
+        b = min(a + step, b);
     }
     u.s = a;
     const uint32_t head = (pl.prefix[a + 1] - pl.prefix[a]) / (uint32_t)p.kv.n_kv;
@@ -294,12 +294,22 @@ FDEV void attn_unit_find(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
     u.g = (int)(rem / head);
     rem -= (uint32_t)u.g * head;
     const int4 q = pl.seq[a];
-    u.i = 0;
-    for (;;) {
-        const uint32_t n = attn_steps(q.y, q.z, p, ru, bk_shift, u.i);
-        if (rem < n) break;
-        rem -= n;
-        u.i++;
+    const int nu = fdiv(q.y * p.group + ru - 1, p.by_ru);
+    for (int i0 = 0;; i0 += 32) {
+        uint32_t n = i0 + lane < nu ? attn_steps(q.y, q.z, p, ru, bk_shift, i0 + lane) : 0, sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += t;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, sum > rem);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            rem -= __shfl_sync(0xffffffffu, sum - n, l);
+            u.i = i0 + l;
+            break;
+        }
+        rem -= __shfl_sync(0xffffffffu, sum, 31);
     }
     u.u0 = x - rem;
     attn_unit_fill(u, pl, p, ru, bk_shift);

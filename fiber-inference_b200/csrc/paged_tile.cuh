@@ -9,6 +9,7 @@
 //   warp 8      one lane issues the MMAs: S = Q K^T (operands in shared memory), then
 //               O += P V with P read from tensor memory
 //   warp 9      producer: Q, K and V tiles by TMA (K / V boxes go page by page)
+//   warp 10     scheduler: works out the CTA's units ahead of the others
 // Tensor memory: S_A, S_B (128 columns each; P overwrites the front half of its S), O_A,
 // O_B (head_dim columns each). While one tile's softmax runs, the tensor core works on
 // the other's products.
@@ -24,7 +25,7 @@ namespace fiber {
 
 constexpr int PT_ROWS = 128;                          // rows of a tile
 constexpr int PT_BK_SHIFT = 7, PT_BK = 1 << PT_BK_SHIFT;  // keys of a tile
-constexpr int PT_THREADS = 384;  // three warpgroups; warps 10 and 11 only make up the third
+constexpr int PT_THREADS = 384;  // three warpgroups; warp 11 only makes up the third
 constexpr float PT_GROWTH = 8.f;  // powers of two a row's maximum may grow before O is rescaled
 
 // Tokens and rows of a tile: whole tokens (all heads of the group).
@@ -35,18 +36,35 @@ HDCE int pt_tile_bytes() { return 128 * HD * 2; }  // a Q, K or V tile: [HD / 64
 template <int HD>
 HDCE int pt_stages() { return HD == 128 ? 5 : 8; }
 
+// A unit (or this CTA's piece of it) as the scheduler hands it to the other warps.
+struct PtWork {
+    int q0, slot, g;       // first token row of the sequence, cache slot, KV head
+    int p0;                // position of the sequence's first token
+    int row0, rows[2];     // first row of tile A, rows of tiles A and B
+    int lo, hi;            // positions any row of the unit sees
+    int kt0, b, e;         // key tile of step 0; this piece's steps
+    int ab[2], ae[2];      // steps [ab, ae) in which the tile has work
+    int mode;              // PT_WHOLE, PT_PIECE or PT_END
+    int slot_of, ca, cb;   // piece: its state's place, first and last CTA of the unit
+};
+enum : int { PT_WHOLE = 0, PT_PIECE = 1, PT_END = 2 };
+constexpr int PT_CONSUMERS = 10;  // warps that read the work records
+
 struct PtShared {
     AttnPlan plan;
     uint64_t kvfull[8], kvfree[8];
     uint64_t qfull, qfree;
     uint64_t sfull[2], pready[2], odone[2];
-    uint64_t mdone;
+    uint64_t wfull[2], wfree[2];
+    uint64_t join, mdone;
+    PtWork work[2];
     uint32_t tmem;
     int last;
     int fail;
 };
 template <int HD>
 HDCE int pt_smem() { return (2 + pt_stages<HD>()) * pt_tile_bytes<HD>() + (int)sizeof(PtShared); }
+static_assert(pt_smem<128>() <= 227 * 1024 && pt_smem<64>() <= 227 * 1024, "shared memory of one CTA");
 
 FDEV uint64_t pt_desc(uint32_t saddr, uint32_t lbo) {
     // 128-byte swizzle (2 << 61), version 1, 8-row groups 1024 B apart; lbo: for the operand
@@ -91,7 +109,6 @@ FDEV void pt_commit(uint32_t me, uint64_t *bar) {
 }
 FDEV void pt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 FDEV void pt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-FDEV void pt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 FDEV void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 32 columns of this warp's 32 lanes (one row per thread)
@@ -126,38 +143,63 @@ FDEV float pt_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two fp32 values in one 64-bit register
+FDEV uint64_t pt_two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+FDEV float2 pt_both(uint64_t r) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
+    return f;
+}
+FDEV uint64_t pt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+FDEV uint64_t pt_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (added and
+// subtracted 1.5 * 2^23), 2^f by a minimax polynomial of degree 4 on [-1/2, 1/2] (Remez
+// exchange on the relative error, 2.7e-6 in fp32), n added to the exponent. x is clamped
+// to -126: what lies below is nothing beside the row's largest weight of at least 1.
+FDEV float2 pt_exp2_poly(float x0, float x1) {
+    const uint64_t magic = pt_two(12582912.f, 12582912.f), minus = pt_two(-12582912.f, -12582912.f);
+    const uint64_t x = pt_two(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+    const uint64_t t = pt_add2(x, magic);
+    const uint64_t n = pt_add2(t, minus);
+    const uint64_t f = pt_fma2(n, pt_two(-1.f, -1.f), x);
+    uint64_t y = pt_fma2(pt_two(0.009570102207362652f, 0.009570102207362652f), f, pt_two(0.05591785907745361f, 0.05591785907745361f));
+    y = pt_fma2(y, f, pt_two(0.240247443318367f, 0.240247443318367f));
+    y = pt_fma2(y, f, pt_two(0.6931217908859253f, 0.6931217908859253f));
+    y = pt_fma2(y, f, pt_two(0.9999992847442627f, 0.9999992847442627f));
+    const float2 v = pt_both(y), e = pt_both(t);
+    return make_float2(__uint_as_float(__float_as_uint(v.x) + (__float_as_uint(e.x) << 23)),
+                       __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(e.y) << 23)));
+}
+// Completion of tensor-memory loads, tied to the registers they fill
+FDEV void pt_wait_ld(float *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 :
+                 : "memory");
+}
+FDEV void pt_tie16(float *v) {
+    asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                      "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+}
 // The lowest n bits (none below 0, all from 32)
 FDEV uint32_t pt_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
-FDEV void pt_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// A unit's piece [b, e) of steps, as every warp of the CTA sees it.
-struct PtPiece {
-    uint32_t b, e;
-    int kt0;       // key tile of step 0
-    int rows[2];   // rows of tile A, B
-    int ab[2], ae[2];  // steps [ab, ae) in which the tile has work
-};
-FDEV void pt_piece(PtPiece &q, const AttnUnit &u, const AttnPagedParams &p, int rt, uint32_t x, uint32_t x1) {
-    q.b = x - u.u0;
-    q.e = min(x1 - u.u0, u.steps);
-    q.kt0 = u.lo >> PT_BK_SHIFT;
-    const bool any = u.hi > u.lo;
-    q.rows[0] = min(rt, u.rows);
-    q.rows[1] = u.rows - q.rows[0];
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        int lo = 0, hi = 0;
-        if (q.rows[t] > 0 && any) attn_span(u.nq, u.kv, p, u.row0 + t * rt, q.rows[t], lo, hi);
-        if (hi > lo) {
-            q.ab[t] = max((int)q.b, (lo >> PT_BK_SHIFT) - q.kt0);
-            q.ae[t] = min((int)q.e, ((hi + PT_BK - 1) >> PT_BK_SHIFT) - q.kt0);
-        } else {
-            q.ab[t] = q.ae[t] = 0;
-        }
-        if (q.ae[t] < q.ab[t]) q.ae[t] = q.ab[t];
-    }
-}
-FDEV bool pt_on(const PtPiece &q, int t, int k) { return k >= q.ab[t] && k < q.ae[t]; }
+// Pairs of every 4 whose exponentials run on the FMA pipe instead of the special-function
+// unit, which alone would need 2 x 1,024 cycles per step beside 2,048 of the tensor core.
+constexpr int PT_POLY = 1;
 
 template <int HD, bool BF>
 __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_constant__ AttnPagedParams p) {
@@ -181,51 +223,101 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
             pg_init(&sh.sfull[t], 1);
             pg_init(&sh.pready[t], 4);
             pg_init(&sh.odone[t], 1);
+            pg_init(&sh.wfull[t], 1);
+            pg_init(&sh.wfree[t], PT_CONSUMERS);
         }
+        pg_init(&sh.join, 8);
         pg_init(&sh.mdone, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.fail = 0;
     }
-    pdl_trigger();
-    pdl_wait();
-    const int rt = pt_tile_rows(p.group), ru = 2 * rt;
-    const uint32_t total = attn_plan_build<PT_THREADS>(sh.plan, p, ru, PT_BK_SHIFT);
-    const int n_cta = min((int)gridDim.x, (int)min(total, 0x7fffffffu)), cta = blockIdx.x;
-    if (cta >= n_cta) return;
-    const uint32_t x0 = attn_share(total, n_cta, cta), x1 = attn_share(total, n_cta, cta + 1);
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pg_saddr(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    pdl_trigger();
+    pdl_wait();
+    const int rt = pt_tile_rows(p.group), ru = 2 * rt;
     pt_fence_before();
-    __syncthreads();
+    const uint32_t total = attn_plan_build<PT_THREADS>(sh.plan, p, ru, PT_BK_SHIFT);  // ends with a barrier
     pt_fence_after();
-    if (sh.tmem != 0 && tid == 0) *p.status = 2;  // never: all 512 columns start at column 0
-    constexpr uint32_t tmem = 0;
-    AttnUnit u;
-    attn_unit_find(u, sh.plan, p, ru, PT_BK_SHIFT, x0);
-    PtPiece q;
+    constexpr uint32_t tmem = 0;  // all 512 columns
+    if (sh.tmem != tmem && tid == 0) *p.status = 2;
+    const int n_cta = min((int)gridDim.x, (int)min(total, 0x7fffffffu)), cta = blockIdx.x;
+
     // 384 threads at 168 registers: the softmax warpgroups take 224 each, the third keeps 56
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 9) {
+        if (cta < n_cta && warp == 10) {
+            // ---- scheduler
+            const uint32_t x1 = attn_share(total, n_cta, cta + 1);
+            uint32_t x = attn_share(total, n_cta, cta);
+            AttnUnit u;
+            attn_unit_find(u, sh.plan, p, ru, PT_BK_SHIFT, x);
+            for (uint32_t i = 0;; i++) {
+                bool ok = i < 2 || pg_wait(&sh.wfree[i & 1], ((i >> 1) - 1) & 1, &sh.fail);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                PtWork &w = sh.work[i & 1];
+                const bool end = x >= x1;
+                const int b = (int)(x - u.u0), e = (int)min(x1 - u.u0, u.steps), kt0 = u.lo >> PT_BK_SHIFT;
+                if (lane < 2 && !end) {  // lane t: tile t
+                    const int rows = lane == 0 ? min(rt, u.rows) : max(0, u.rows - rt);
+                    int lo = 0, hi = 0, ab = 0, ae = 0;
+                    if (rows > 0 && u.hi > u.lo) attn_span(u.nq, u.kv, p, u.row0 + lane * rt, rows, lo, hi);
+                    if (hi > lo) {
+                        ab = max(b, (lo >> PT_BK_SHIFT) - kt0);
+                        ae = max(ab, min(e, ((hi + PT_BK - 1) >> PT_BK_SHIFT) - kt0));
+                    }
+                    w.rows[lane] = rows;
+                    w.ab[lane] = ab;
+                    w.ae[lane] = ae;
+                }
+                if (lane == 0) {
+                    w.mode = end ? PT_END : (b == 0 && e == (int)u.steps ? PT_WHOLE : PT_PIECE);
+                    if (!end) {
+                        w.q0 = u.q0;
+                        w.slot = u.slot;
+                        w.g = u.g;
+                        w.p0 = u.kv - u.nq;
+                        w.row0 = u.row0;
+                        w.lo = u.lo;
+                        w.hi = u.hi;
+                        w.kt0 = kt0;
+                        w.b = b;
+                        w.e = e;
+                        w.slot_of = 2 * cta + (b > 0 ? 0 : 1);
+                        w.ca = attn_owner(total, n_cta, u.u0);
+                        w.cb = attn_owner(total, n_cta, u.u0 + u.steps - 1);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) pg_arrive(&sh.wfull[i & 1]);
+                if (end) break;
+                x = u.u0 + (uint32_t)e;
+                if (x < x1) attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+            }
+        } else if (cta < n_cta && warp == 9) {
             // ---- producer: lane b issues box b of a K or V tile
             const int box_rows = min(1 << p.kv.page_shift, PT_BK), nrb = PT_BK / box_rows;
             const int half = lane / nrb, rb = lane % nrb, mask = (1 << p.kv.page_shift) - 1;
             const bool boxed = lane < HALVES * nrb;
             const uint32_t dst0 = half * (128 * 128) + rb * box_rows * 128;
             uint32_t it = 0, nq = 0;  // K / V tiles and Q pairs issued
-            bool ok = true;
-            for (uint32_t x = x0;;) {
-                pt_piece(q, u, p, rt, x, x1);
-                if (q.ae[0] > q.ab[0] || q.ae[1] > q.ab[1]) {
-                    const int32_t *tab = p.kv.table + (long long)u.slot * p.kv.max_pages;
-                    const int used = (u.hi + mask) >> p.kv.page_shift;
-                    for (uint32_t k = q.b; k < q.e; k++) {
-                        const int key = ((q.kt0 + (int)k) << PT_BK_SHIFT) + rb * box_rows, lp = key >> p.kv.page_shift;
+            for (uint32_t i = 0;; i++) {
+                bool ok = pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const PtWork &w = sh.work[i & 1];
+                if (w.mode == PT_END) break;
+                if (w.ae[0] > w.ab[0] || w.ae[1] > w.ab[1]) {
+                    const int32_t *tab = p.kv.table + (long long)w.slot * p.kv.max_pages;
+                    const int used = (w.hi + mask) >> p.kv.page_shift, e = w.e, g = w.g;
+                    for (int k = w.b; k < e; k++) {
+                        const int key = ((w.kt0 + k) << PT_BK_SHIFT) + rb * box_rows, lp = key >> p.kv.page_shift;
                         int page = p.kv.n_pages;  // outside the tensor: reads as zeros
                         if (boxed && lp < used) page = tab[lp];
-    #pragma unroll
+#pragma unroll
                         for (int v = 0; v < 2; v++, it++) {
                             const int st = it % NST;
                             if (it >= NST) ok = pg_wait(&sh.kvfree[st], (it / NST - 1) & 1, &sh.fail);
@@ -234,46 +326,44 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                             if (lane == 0) pg_expect_tx(&sh.kvfull[st], TB);
                             __syncwarp();
                             if (boxed)
-                                pg_tma4(pg_saddr(ring + st * TB) + dst0, v ? &p.vmap : &p.kmap, half * 64, key & mask, u.g, page,
+                                pg_tma4(pg_saddr(ring + st * TB) + dst0, v ? &p.vmap : &p.kmap, half * 64, key & mask, g, page,
                                         &sh.kvfull[st]);
                         }
                         if (!ok) break;
-                        if (k == q.b) {  // the queries' buffer is free last: K and V of the first step go before
+                        if (k == w.b) {  // the queries' buffer is free last: K and V of the first step go before
                             if (nq > 0) ok = pg_wait(&sh.qfree, (nq - 1) & 1, &sh.fail);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
                             if (lane == 0) {
-                                const int nt = q.rows[1] > 0 ? 2 : 1;
+                                const int nt = w.rows[1] > 0 ? 2 : 1;
                                 pg_expect_tx(&sh.qfull, (uint32_t)(nt * HALVES * rt * 128));
                                 for (int t = 0; t < nt; t++)
                                     for (int h = 0; h < HALVES; h++)
-                                        pg_tma3(pg_saddr(qbuf + t * TB) + h * (128 * 128), &p.qmap, 64 * h, u.g * p.group,
-                                                u.q0 + fdiv(u.row0 + t * rt, p.by_group), &sh.qfull);
+                                        pg_tma3(pg_saddr(qbuf + t * TB) + h * (128 * 128), &p.qmap, 64 * h, g * p.group,
+                                                w.q0 + fdiv(w.row0 + t * rt, p.by_group), &sh.qfull);
                             }
                             nq++;
                         }
                     }
+                    if (!ok) break;
                 }
-                x = u.u0 + q.e;
-                if (!ok || x >= x1) break;
-                attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+                __syncwarp();
+                if (lane == 0) pg_arrive(&sh.wfree[i & 1]);
             }
             if (lane == 0) {  // every copy has landed before the CTA exits
                 for (uint32_t s = 0; s < NST && s < it; s++)
                     pg_wait(&sh.kvfull[s], (s + (it - 1 - s) / NST * NST) / NST & 1, nullptr);
                 if (nq > 0) pg_wait(&sh.qfull, (nq - 1) & 1, nullptr);
             }
-        } else if (warp == 8) {
+        } else if (cta < n_cta && warp == 8) {
             // ---- MMA issuer
             constexpr uint32_t IS = pt_idesc<BF>(PT_BK, false), IO = pt_idesc<BF>(HD, true);
             const uint32_t me = pt_elect();
             uint32_t nq = 0, np[2] = {0, 0};
             int ks = 0, kph = 0;  // ring stage and parity of step k's K tile; its V tile is the next
-            bool ok = true;
-            auto after = [&](int &st, int &ph, int n) {
-                st += n;
-                if (st >= NST) {
-                    st -= NST;
+            auto after = [&](int &st, int &ph) {
+                if (++st == NST) {
+                    st = 0;
                     ph ^= 1;
                 }
             };
@@ -282,7 +372,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++) {
                     const uint32_t o = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-                    pt_mma_ss(me, t * 128, a + o, b + o, IS, k > 0);
+                    pt_mma_ss(me, tmem + t * 128, a + o, b + o, IS, k > 0);
                 }
                 pt_commit(me, &sh.sfull[t]);
             };
@@ -290,99 +380,138 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 const uint64_t b = pt_desc(pg_saddr(ring) + st * TB, 128 * 128);
 #pragma unroll
                 for (int k = 0; k < PT_BK / 16; k++)
-                    pt_mma_ts(me, 256 + t * 128, t * 128 + 8 * k, b + k * (2048 >> 4), IO, !first || k > 0);
+                    pt_mma_ts(me, tmem + 256 + t * 128, tmem + t * 128 + 8 * k, b + k * (2048 >> 4), IO, !first || k > 0);
             };
-            for (uint32_t x = x0; ok;) {
-                pt_piece(q, u, p, rt, x, x1);
-                if (q.ae[0] > q.ab[0] || q.ae[1] > q.ab[1]) {
-                    ok = pg_wait(&sh.qfull, nq & 1, &sh.fail) && pg_wait(&sh.kvfull[ks], kph, &sh.fail);
+            for (uint32_t i = 0;; i++) {
+                bool ok = pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const PtWork &w = sh.work[i & 1];
+                if (w.mode == PT_END) break;
+                const int b = w.b, e = w.e, ab0 = w.ab[0], ab1 = w.ab[1], ae0 = w.ae[0], ae1 = w.ae[1];
+                __syncwarp();
+                if (lane == 0) pg_arrive(&sh.wfree[i & 1]);
+                if (ae0 <= ab0 && ae1 <= ab1) continue;
+                auto on = [&](int t, int k) { return t == 0 ? k >= ab0 && k < ae0 : k >= ab1 && k < ae1; };
+                ok = pg_wait(&sh.qfull, nq & 1, &sh.fail) && pg_wait(&sh.kvfull[ks], kph, &sh.fail);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                nq++;
+                pt_fence_after();
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+                    if (on(t, b)) scores(t, ks);
+                pt_commit(me, &sh.kvfree[ks]);
+                if (e - b == 1) pt_commit(me, &sh.qfree);
+                for (int k = b; k < e; k++) {
+                    const bool more = k + 1 < e;
+                    int vs = ks, vph = kph;
+                    after(vs, vph);
+                    int ns = vs, nph = vph;  // the next step's K tile
+                    after(ns, nph);
+                    if (more) ok = pg_wait(&sh.kvfull[ns], nph, &sh.fail);
+                    ok = ok && pg_wait(&sh.kvfull[vs], vph, &sh.fail);
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        if (on(t, k)) {
+                            ok = ok && pg_wait(&sh.pready[t], np[t] & 1, &sh.fail);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            np[t]++;
+                            pt_fence_after();
+                            values(t, vs, k == (t == 0 ? ab0 : ab1));
+                            if (k + 1 == (t == 0 ? ae0 : ae1)) pt_commit(me, &sh.odone[t]);
+                        }
+                        if (t == 1) pt_commit(me, &sh.kvfree[vs]);
+                        if (more && on(t, k + 1)) scores(t, ns);
+                    }
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    nq++;
-                    pt_fence_after();
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-                        if (pt_on(q, t, q.b)) scores(t, ks);
-                    pt_commit(me, &sh.kvfree[ks]);
-                    if (q.e - q.b == 1) pt_commit(me, &sh.qfree);
-                    for (int k = q.b; k < (int)q.e; k++) {
-                        const bool more = k + 1 < (int)q.e;
-                        int vs = ks, vph = kph;
-                        after(vs, vph, 1);
-                        int ns = vs, nph = vph;  // the next step's K tile
-                        after(ns, nph, 1);
-                        if (more) ok = pg_wait(&sh.kvfull[ns], nph, &sh.fail);
-                        ok = ok && pg_wait(&sh.kvfull[vs], vph, &sh.fail);
-#pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            if (pt_on(q, t, k)) {
-                                ok = ok && pg_wait(&sh.pready[t], np[t] & 1, &sh.fail);
-                                ok = __all_sync(0xffffffffu, ok);
-                                if (!ok) break;
-                                np[t]++;
-                                pt_fence_after();
-                                values(t, vs, k == q.ab[t]);
-                                if (k + 1 == q.ae[t]) pt_commit(me, &sh.odone[t]);
-                            }
-                            if (t == 1) pt_commit(me, &sh.kvfree[vs]);
-                            if (more && pt_on(q, t, k + 1)) scores(t, ns);
-                        }
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        if (more) pt_commit(me, &sh.kvfree[ns]);
-                        if (k + 2 == (int)q.e) pt_commit(me, &sh.qfree);
-                        ks = ns;
-                        kph = nph;
-                    }
+                    if (more) pt_commit(me, &sh.kvfree[ns]);
+                    if (k + 2 == e) pt_commit(me, &sh.qfree);
+                    ks = ns;
+                    kph = nph;
                 }
-                x = u.u0 + q.e;
-                if (x >= x1) break;
-                attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+                if (!ok) break;
             }
             pt_commit(me, &sh.mdone);  // every product has finished before tensor memory is released
             pg_wait(&sh.mdone, 0, nullptr);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-        // ---- softmax: thread = row of tile t
+        // ---- softmax: thread = row of tile t. After a timed-out wait these warps run through
+        // (the status says so), so that every barrier is met.
         const int t = warp >> 2, row = tid & 127;
         const uint32_t sa = tmem + t * 128 + ((uint32_t)(32 * (warp & 3)) << 16), oa = sa + 256;
-        uint32_t it = 0, ns = 0, no = 0;
-        for (uint32_t x = x0;;) {
-            pt_piece(q, u, p, rt, x, x1);
-            const bool whole = q.b == 0 && q.e == u.steps;
-            const bool run = q.ae[0] > q.ab[0] || q.ae[1] > q.ab[1];
-            const int p0 = u.kv - u.nq, tok = fdiv(u.row0 + t * rt + row, p.by_group), head = u.g * p.group + u.row0 + t * rt + row - tok * p.group;
-            const bool in = row < q.rows[t];
-            const int rhi = in ? p0 + tok + 1 : 0, rlo = p.window > 0 ? max(0, p0 + tok - p.window + 1) : 0;
-            // every row of the tile sees the keys in [all_lo, all_hi)
-            const int all_hi = q.rows[t] > 0 ? p0 + fdiv(u.row0 + t * rt, p.by_group) + 1 : 0;
-            const int all_lo = p.window > 0 && q.rows[t] > 0 ? max(0, p0 + fdiv(u.row0 + t * rt + q.rows[t] - 1, p.by_group) - p.window + 1) : 0;
+        const uint64_t scale2 = pt_two(p.scale_log2, p.scale_log2);
+        uint32_t it = 0, ns = 0, no = 0, nj = 0;
+        for (uint32_t i = 0; cta < n_cta; i++) {
+            if (!__all_sync(0xffffffffu, pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail))) break;
+            const PtWork &w = sh.work[i & 1];
+            const int mode = w.mode;
+            if (mode == PT_END) break;
+            const int rows = w.rows[t], row0 = w.row0 + t * rt, ab = w.ab[t], ae = w.ae[t];
+            int rlo, rhi, all_lo = 0, all_hi;  // positions this row sees; those every row of the tile sees
+            {
+                const int tok = fdiv(row0 + row, p.by_group);
+                rhi = row < rows ? max(0, w.p0 + tok + 1) : 0;
+                rlo = p.window > 0 ? max(0, w.p0 + tok - p.window + 1) : 0;
+                all_hi = w.p0 + fdiv(row0, p.by_group) + 1;
+                if (p.window > 0) all_lo = max(0, w.p0 + fdiv(row0 + rows - 1, p.by_group) - p.window + 1);
+            }
+            const bool idle = 32 * (warp & 3) >= rows;  // no row of this warp exists: it only keeps step
             float m = -INFINITY, l = 0.f;
-            if (run) {
-                for (int k = q.b; k < (int)q.e; k++, it += 2) {
-                    if (!pt_on(q, t, k)) continue;
-                    const int key0 = (q.kt0 + k) << PT_BK_SHIFT;
-                    pg_wait(&sh.sfull[t], ns & 1, &sh.fail);  // after a timeout: runs through, status says so
-                    ns++;
-                    pt_fence_after();
+            for (int k = ab; k < ae; k++) {
+                const int key0 = (w.kt0 + k) << PT_BK_SHIFT;
+                pg_wait(&sh.sfull[t], ns & 1, &sh.fail);
+                ns++;
+                pt_fence_after();
+                if (!idle) {
                     float s[128];
+                    pt_ld32(s, sa);
+                    pt_ld32(s + 32, sa + 32);
+                    pt_wait_ld(s);
+                    pt_tie16(s + 16);
+                    pt_tie16(s + 32);
+                    pt_tie16(s + 48);
+                    pt_ld32(s + 64, sa + 64);
+                    pt_ld32(s + 96, sa + 96);
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
+                    const bool masked = key0 < all_lo || key0 + PT_BK > all_hi;
+                    const int ca = rlo - key0, cb = rhi - key0;  // columns [ca, cb) are seen
+                    if (masked) {
 #pragma unroll
-                    for (int c = 0; c < 128; c += 32) pt_ld32(s + c, sa + c);
-                    pt_wait_ld();
-                    if (key0 < all_lo || key0 + PT_BK > all_hi) {
-                        const int a = rlo - key0, b = rhi - key0;  // columns [a, b) are seen
+                        for (int c = 0; c < 64; c += 32) {
+                            const uint32_t keep = pt_below(cb - c) & ~pt_below(ca - c);
 #pragma unroll
-                        for (int c = 0; c < 128; c += 32) {
-                            const uint32_t keep = pt_below(b - c) & ~pt_below(a - c);
+                            for (int j = 0; j < 32; j++)
+                                if (!(keep >> j & 1)) s[c + j] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 4; c++) mx[c] = s[c];
+                    }
+#pragma unroll
+                    for (int c = 4; c < 64; c += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            mx[j] = c + 4 + j < 64 ? fmaxf(fmaxf(mx[j], s[c + j]), s[c + 4 + j]) : fmaxf(mx[j], s[c + j]);
+                    pt_wait_ld(s + 64);
+                    pt_tie16(s + 80);
+                    pt_tie16(s + 96);
+                    pt_tie16(s + 112);
+                    if (masked) {
+#pragma unroll
+                        for (int c = 64; c < 128; c += 32) {
+                            const uint32_t keep = pt_below(cb - c) & ~pt_below(ca - c);
 #pragma unroll
                             for (int j = 0; j < 32; j++)
                                 if (!(keep >> j & 1)) s[c + j] = -INFINITY;
                         }
                     }
-                    float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                    for (int c = 64; c < 128; c += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) mx[j] = fmaxf(fmaxf(mx[j], s[c + j]), s[c + 4 + j]);
                     const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
                     const bool grow = mt > m + PT_GROWTH || (m == -INFINITY && mt > m);
                     if (__any_sync(0xffffffffu, grow)) {
@@ -390,89 +519,102 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                         const float f = grow ? pt_exp2(m - mn) : 1.f;
                         m = mn;
                         l *= f;
-                        if (k > q.ab[t]) {
+                        if (k > ab) {
 #pragma unroll
                             for (int c = 0; c < HD; c += 16) {
                                 float o[16];
-                                uint32_t w[16];
+                                uint32_t x[16];
                                 pt_ld16(o, oa + c);
-                                pt_wait_ld();
+                                pt_wait_ld(o);
 #pragma unroll
-                                for (int j = 0; j < 16; j++) w[j] = __float_as_uint(o[j] * f);
-                                pt_st16(oa + c, w);
+                                for (int j = 0; j < 16; j++) x[j] = __float_as_uint(o[j] * f);
+                                pt_st16(oa + c, x);
                             }
                         }
                     }
-                    const float base = m == -INFINITY ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float nb = m == -INFINITY ? 0.f : -m;
+                    const uint64_t nb2 = pt_two(nb, nb);
+                    uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
                     for (int c = 0; c < 128; c += 32) {
-                        uint32_t w[16];
+                        uint32_t x[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            const float a = pt_exp2(fmaf(s[c + 2 * j], p.scale_log2, -base));
-                            const float b = pt_exp2(fmaf(s[c + 2 * j + 1], p.scale_log2, -base));
-                            sum[(2 * j) & 3] += a;
-                            sum[(2 * j + 1) & 3] += b;
-                            w[j] = pack2<BF>(a, b);
+                            float2 y = pt_both(pt_fma2(pt_two(s[c + 2 * j], s[c + 2 * j + 1]), scale2, nb2));
+                            if ((j & 3) < 4 - PT_POLY) {
+                                y.x = pt_exp2(y.x);
+                                y.y = pt_exp2(y.y);
+                            } else {
+                                y = pt_exp2_poly(y.x, y.y);
+                            }
+                            sum[j & 1] = pt_add2(sum[j & 1], pt_two(y.x, y.y));
+                            x[j] = pack2<BF>(y.x, y.y);
                         }
-                        pt_st16(sa + c / 2, w);
+                        pt_st16(sa + c / 2, x);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    if ((key0 < u.lo || key0 + PT_BK > u.hi) && (t == 0 || !pt_on(q, 0, k))) {
-                        // values no row of the unit sees may hold anything: weight 0 must meet 0 there
-                        const uint32_t vi = it + 1;
-                        pg_wait(&sh.kvfull[vi % NST], vi / NST & 1, &sh.fail);
-                        if (key0 + row < u.lo || key0 + row >= u.hi)
-#pragma unroll 1
-                            for (int c = 0; c < 8 * HALVES; c++)  // pieces rotated by the row: eight rows on eight banks
-                                *reinterpret_cast<uint4 *>(ring + (vi % NST) * TB + (c >> 3) * (128 * 128) + row * 128 +
-                                                           (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-                        pg_proxy_fence();
-                    }
-                    pt_wait_st();
-                    pt_fence_before();
-                    __syncwarp();
-                    if (lane == 0) pg_arrive(&sh.pready[t]);
+                    const float2 l2 = pt_both(pt_add2(sum[0], sum[1]));
+                    l += l2.x + l2.y;
                 }
+                if ((key0 < w.lo || key0 + PT_BK > w.hi) && (t == 0 || k < w.ab[0] || k >= w.ae[0])) {
+                    // values no row of the unit sees may hold anything: weight 0 must meet 0 there
+                    const uint32_t vi = it + 2 * (k - w.b) + 1;
+                    pg_wait(&sh.kvfull[vi % NST], vi / NST & 1, &sh.fail);
+                    if (key0 + row < w.lo || key0 + row >= w.hi)
+#pragma unroll 1
+                        for (int c = 0; c < 8 * HALVES; c++)  // pieces rotated by the row: eight rows on eight banks
+                            *reinterpret_cast<uint4 *>(ring + (vi % NST) * TB + (c >> 3) * (128 * 128) + row * 128 +
+                                                       (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                    pg_proxy_fence();
+                }
+                pt_wait_st();
+                pt_fence_before();
+                __syncwarp();
+                if (lane == 0) pg_arrive(&sh.pready[t]);
             }
             // ---- the unit's (or piece's) output
-            const bool did = q.ae[t] > q.ab[t];
+            if (w.ae[0] > w.ab[0] || w.ae[1] > w.ab[1]) it += 2 * (w.e - w.b);
+            const bool did = ae > ab;
             if (did) {
                 pg_wait(&sh.odone[t], no & 1, &sh.fail);
                 no++;
                 pt_fence_after();
             }
-            uint16_t *dst = p.out + (long long)(u.q0 + tok) * p.ldo + (long long)head * HD;
+            const int tok = fdiv(row0 + row, p.by_group), head = w.g * p.group + row0 + row - tok * p.group;
+            uint16_t *dst = p.out + (long long)(w.q0 + tok) * p.ldo + (long long)head * HD;
             bool bad = false;
-            auto store32 = [&](int c, const float *o) {  // 32 output values of this thread's row
+            auto store16 = [&](int c, const float *o) {  // 16 output values of this thread's row
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
+                for (int j = 0; j < 16; j += 8) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) bad |= !isfinite(o[j + i]);
+                    for (int i2 = 0; i2 < 8; i2++) bad |= !isfinite(o[j + i2]);
                     *reinterpret_cast<uint4 *>(dst + c + j) =
                         make_uint4(pack2<BF>(o[j], o[j + 1]), pack2<BF>(o[j + 2], o[j + 3]), pack2<BF>(o[j + 4], o[j + 5]),
                                    pack2<BF>(o[j + 6], o[j + 7]));
                 }
             };
-            if (whole) {
+            if (mode == PT_WHOLE) {
                 const float inv = 1.f / l;
+                if (!idle)
 #pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    float o[32];
-                    if (did) {
-                        pt_ld32(o, oa + c);
-                        pt_wait_ld();
+                    for (int c = 0; c < HD; c += 32) {
+                        float o[32];
+                        if (did) {
+                            pt_ld32(o, oa + c);
+                            pt_wait_ld(o);
+                            pt_tie16(o + 16);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j++) o[j] = did && rhi > rlo ? o[j] * inv : 0.f;
+                        if (row < rows) {
+                            store16(c, o);
+                            store16(c + 16, o + 16);
+                        }
                     }
-#pragma unroll
-                    for (int j = 0; j < 32; j++) o[j] = did && rhi > rlo ? o[j] * inv : 0.f;
-                    if (in) store32(c, o);
-                }
             } else {
-                const int pslot = 2 * cta + (q.b > 0 ? 0 : 1);
-                float4 *po = reinterpret_cast<float4 *>(p.part_o) + (long long)(2 * pslot + t) * (HD / 4) * 128 + row;
-                float *pm = p.part_ml + (2 * pslot + t) * 256 + row;
-                if (q.rows[t] > 0) {
+                const int ps = 2 * w.slot_of + t;
+                float4 *po = reinterpret_cast<float4 *>(p.part_o) + (long long)ps * (HD / 4) * 128 + row;
+                float *pm = p.part_ml + ps * 256 + row;
+                if (!idle) {
                     pm[0] = did ? m : -INFINITY;
                     pm[128] = l;
                     if (did)
@@ -480,39 +622,39 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                         for (int c = 0; c < HD; c += 32) {
                             float o[32];
                             pt_ld32(o, oa + c);
-                            pt_wait_ld();
+                            pt_wait_ld(o);
+                            pt_tie16(o + 16);
 #pragma unroll
                             for (int j = 0; j < 32; j += 4) po[(c + j) / 4 * 128] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                         }
                 }
-                const int ca = attn_owner(total, n_cta, u.u0), cb = attn_owner(total, n_cta, u.u0 + u.steps - 1);
                 __threadfence();
-                pt_bar();
+                __syncwarp();
+                if (lane == 0) pg_arrive(&sh.join);
+                pg_wait(&sh.join, nj++ & 1, &sh.fail);
                 if (tid == 0) {
-                    sh.last = atomicAdd(&p.tickets[ca], 1u) == (unsigned)(cb - ca);
-                    if (sh.last) p.tickets[ca] = 0u;
+                    sh.last = atomicAdd(&p.tickets[w.ca], 1u) == (unsigned)(w.cb - w.ca);
+                    if (sh.last) p.tickets[w.ca] = 0u;
                     __threadfence();
                 }
-                pt_bar();
-                if (sh.last && q.rows[t] > 0) {
+                __syncwarp();
+                if (lane == 0) pg_arrive(&sh.join);
+                pg_wait(&sh.join, nj++ & 1, &sh.fail);
+                if (sh.last && !idle) {
+                    const int c0 = w.ca, c1 = w.cb;
                     float M = -INFINITY, L = 0.f;
-                    for (int c = ca; c <= cb; c++)
-                        M = fmaxf(M, __ldcg(p.part_ml + (2 * (2 * c + (c == ca)) + t) * 256 + row));
-                    for (int c = ca; c <= cb; c++) {
-                        const float *ml = p.part_ml + (2 * (2 * c + (c == ca)) + t) * 256 + row;
-                        const float mc = __ldcg(ml);
-                        if (mc != -INFINITY) L = fmaf(pt_exp2(mc - M), __ldcg(ml + 128), L);
-                    }
-                    const float inv = rhi > rlo ? 1.f / L : 0.f;
+                    for (int c = c0; c <= c1; c++)
+                        M = fmaxf(M, __ldcg(p.part_ml + (2 * (2 * c + (c == c0)) + t) * 256 + row));
                     float o[HD];
 #pragma unroll
                     for (int j = 0; j < HD; j++) o[j] = 0.f;
 #pragma unroll 1
-                    for (int c = ca; c <= cb; c++) {
-                        const int sl = 2 * (2 * c + (c == ca)) + t;
-                        const float mc = __ldcg(p.part_ml + sl * 256 + row);
+                    for (int c = c0; c <= c1; c++) {
+                        const int sl = 2 * (2 * c + (c == c0)) + t;
+                        const float mc = __ldcg(p.part_ml + sl * 256 + row), lc = __ldcg(p.part_ml + sl * 256 + 128 + row);
                         const float4 *src = reinterpret_cast<const float4 *>(p.part_o) + (long long)sl * (HD / 4) * 128 + row;
                         const float f = pt_exp2(mc - M);
+                        if (mc != -INFINITY) L = fmaf(f, lc, L);
 #pragma unroll
                         for (int j0 = 0; j0 < HD / 4; j0 += 16) {
                             float4 v[16];
@@ -529,12 +671,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                                 }
                         }
                     }
-                    if (in)
+                    const float inv = 1.f / L;
+                    if (row < rows)
 #pragma unroll
-                        for (int c = 0; c < HD; c += 32) {
+                        for (int c = 0; c < HD; c += 16) {
 #pragma unroll
-                            for (int j = 0; j < 32; j++) o[c + j] = rhi > rlo ? o[c + j] * inv : 0.f;
-                            store32(c, o + c);
+                            for (int j = 0; j < 16; j++) o[c + j] = rhi > rlo ? o[c + j] * inv : 0.f;
+                            store16(c, o + c);
                         }
                 }
             }
@@ -544,13 +687,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 const int src = __ffs(again) - 1;
                 again &= again - 1;
                 const int stok = __shfl_sync(0xffffffffu, tok, src), shead = __shfl_sync(0xffffffffu, head, src);
-                attn_row_exact<HD, BF>(p, p.q + (long long)(u.q0 + stok) * p.ldq + (long long)shead * HD,
-                                       p.out + (long long)(u.q0 + stok) * p.ldo + (long long)shead * HD, u.slot, u.g,
+                attn_row_exact<HD, BF>(p, p.q + (long long)(w.q0 + stok) * p.ldq + (long long)shead * HD,
+                                       p.out + (long long)(w.q0 + stok) * p.ldo + (long long)shead * HD, w.slot, w.g,
                                        __shfl_sync(0xffffffffu, rlo, src), __shfl_sync(0xffffffffu, rhi, src), lane);
             }
-            x = u.u0 + q.e;
-            if (x >= x1) break;
-            attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+            __syncwarp();
+            if (lane == 0) pg_arrive(&sh.wfree[i & 1]);
         }
     }
     pt_fence_before();
@@ -558,7 +700,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
     if (tid == 0 && sh.fail) *p.status = 1;
     if (warp == 8) {
         pt_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem) : "memory");
     }
 }
 
