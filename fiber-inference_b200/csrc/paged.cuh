@@ -104,14 +104,9 @@ FDEV uint32_t pack2(float a, float b) {  // a in the low half
 
 // ---- mbarriers and TMA -------------------------------------------------------------------
 
-constexpr unsigned long long PG_WAIT_NS = 2000000000ull;
+constexpr long long PG_WAIT_CYCLES = 4000000000ll;  // about 2 s
 
 FDEV uint32_t pg_saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-FDEV unsigned long long pg_now() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
 FDEV void pg_init(uint64_t *bar, int count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(pg_saddr(bar)), "r"(count) : "memory");
 }
@@ -125,21 +120,22 @@ FDEV bool pg_try(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 // Waits for the phase of that parity; gives up when another thread of the CTA has
-// (*fail), or after PG_WAIT_NS (then sets *fail).
-static __device__ __forceinline__ bool pg_wait_slow(uint64_t *bar, uint32_t parity, volatile int *fail) {
-    const unsigned long long t0 = pg_now();
-    for (;;) {
+// (*fail), or after PG_WAIT_CYCLES (then sets *fail). The clock is looked at once in 256
+// tries only: a timer read before the first retry delayed every hand-over that was not
+// ready at once.
+FDEV bool pg_wait(uint64_t *bar, uint32_t parity, volatile int *fail) {
+    long long t0 = 0;
+    for (uint32_t n = 0; !pg_try(bar, parity); n++) {
+        if (n & 255) continue;
         if (fail && *fail) return false;
-        for (int i = 0; i < 64; i++)
-            if (pg_try(bar, parity)) return true;
-        if (pg_now() - t0 > PG_WAIT_NS) {
+        const long long now = clock64();
+        if (n == 0) t0 = now;
+        if (now - t0 > PG_WAIT_CYCLES) {
             if (fail) *fail = 1;
             return false;
         }
     }
-}
-FDEV bool pg_wait(uint64_t *bar, uint32_t parity, volatile int *fail) {
-    return pg_try(bar, parity) || pg_wait_slow(bar, parity, fail);
+    return true;
 }
 FDEV void pg_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pg_saddr(bar)) : "memory");

@@ -6,18 +6,20 @@
 //   warps 0-3   softmax of tile A, one row per thread: scores from tensor memory, running
 //               maximum and sum, probabilities back to tensor memory in 16 bits
 //   warps 4-7   the same for tile B
-//   warp 8      one lane issues the MMAs: S = Q K^T (operands in shared memory), then
-//               O += P V with P read from tensor memory
+//   warps 8, 11 issue the MMAs of tile A and of tile B: S = Q K^T (operands in shared
+//               memory), then O += P V with P read from tensor memory (one warp for both
+//               left the tensor core idle for about 190 cycles at every hand-over)
 //   warp 9      producer: Q, K and V tiles by TMA (K / V boxes go page by page)
 //   warp 10     scheduler: works out the CTA's units ahead of the others
-// Tensor memory: S_A, S_B (128 columns each; P overwrites the front half of its S), O_A,
-// O_B (head_dim columns each). While one tile's softmax runs, the tensor core works on
-// the other's products.
+// Tensor memory: S_A, S_B (128 columns each), O_A, O_B (head_dim columns each). A key tile
+// is worked through in two halves of 64 keys, each with its own 64 columns of S, whose
+// front half its probabilities overwrite: while the softmax of one half runs, the tensor
+// core multiplies the other half's probabilities with V and computes its next scores, so
+// a softmax warp finds its next scores ready. (With one 128-key S per tile a step was the
+// sum of softmax, two products and four hand-overs: 4,200 cycles instead of 2,900.)
 //
 // The output accumulators are rescaled only when a row's maximum has grown by more than
-// 2^8 since the last time (the probabilities, at most 2^8, keep their 11 or 8 bits); the
-// softmax warps do it themselves, since S of the next tile is only reported after the
-// product that last wrote O.
+// 2^8 since the last time (the probabilities, at most 2^8, keep their 11 or 8 bits).
 #pragma once
 #include "paged.cuh"
 
@@ -25,7 +27,7 @@ namespace fiber {
 
 constexpr int PT_ROWS = 128;                          // rows of a tile
 constexpr int PT_BK_SHIFT = 7, PT_BK = 1 << PT_BK_SHIFT;  // keys of a tile
-constexpr int PT_THREADS = 384;  // three warpgroups; warp 11 only makes up the third
+constexpr int PT_THREADS = 384;
 constexpr float PT_GROWTH = 8.f;  // powers of two a row's maximum may grow before O is rescaled
 
 // Tokens and rows of a tile: whole tokens (all heads of the group).
@@ -43,18 +45,19 @@ struct PtWork {
     int row0, rows[2];     // first row of tile A, rows of tiles A and B
     int lo, hi;            // positions any row of the unit sees
     int kt0, b, e;         // key tile of step 0; this piece's steps
-    int ab[2], ae[2];      // steps [ab, ae) in which the tile has work
+    int ab[2], ae[2];      // half steps (64 keys) [ab, ae) in which the tile has work
     int mode;              // PT_WHOLE, PT_PIECE or PT_END
     int slot_of, ca, cb;   // piece: its state's place, first and last CTA of the unit
 };
 enum : int { PT_WHOLE = 0, PT_PIECE = 1, PT_END = 2 };
-constexpr int PT_CONSUMERS = 10;  // warps that read the work records
+constexpr int PT_CONSUMERS = 11;  // warps that read the work records
 
 struct PtShared {
     AttnPlan plan;
     uint64_t kvfull[8], kvfree[8];
     uint64_t qfull, qfree;
-    uint64_t sfull[2], pready[2], odone[2];
+    uint64_t sfull[2][2], pready[2][2];  // [tile][half]
+    uint64_t pvdone[2], odone[2];        // a product with V has finished; a unit's last one has
     uint64_t wfull[2], wfree[2];
     uint64_t join, mdone;
     PtWork work[2];
@@ -215,19 +218,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
     if (tid == 0) {
         for (int s = 0; s < NST; s++) {
             pg_init(&sh.kvfull[s], 1);
-            pg_init(&sh.kvfree[s], 1);
+            pg_init(&sh.kvfree[s], 2);
         }
         pg_init(&sh.qfull, 1);
-        pg_init(&sh.qfree, 1);
+        pg_init(&sh.qfree, 2);
         for (int t = 0; t < 2; t++) {
-            pg_init(&sh.sfull[t], 1);
-            pg_init(&sh.pready[t], 4);
+            for (int h = 0; h < 2; h++) {
+                pg_init(&sh.sfull[t][h], 1);
+                pg_init(&sh.pready[t][h], 4);
+            }
+            pg_init(&sh.pvdone[t], 1);
             pg_init(&sh.odone[t], 1);
             pg_init(&sh.wfull[t], 1);
             pg_init(&sh.wfree[t], PT_CONSUMERS);
         }
         pg_init(&sh.join, 8);
-        pg_init(&sh.mdone, 1);
+        pg_init(&sh.mdone, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.fail = 0;
     }
@@ -266,8 +272,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                     int lo = 0, hi = 0, ab = 0, ae = 0;
                     if (rows > 0 && u.hi > u.lo) attn_span(u.nq, u.kv, p, u.row0 + lane * rt, rows, lo, hi);
                     if (hi > lo) {
-                        ab = max(b, (lo >> PT_BK_SHIFT) - kt0);
-                        ae = max(ab, min(e, ((hi + PT_BK - 1) >> PT_BK_SHIFT) - kt0));
+                        ab = max(2 * b, (lo >> 6) - 2 * kt0);
+                        ae = max(ab, min(2 * e, ((hi + 63) >> 6) - 2 * kt0));
                     }
                     w.rows[lane] = rows;
                     w.ab[lane] = ab;
@@ -355,32 +361,35 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                     pg_wait(&sh.kvfull[s], (s + (it - 1 - s) / NST * NST) / NST & 1, nullptr);
                 if (nq > 0) pg_wait(&sh.qfull, (nq - 1) & 1, nullptr);
             }
-        } else if (cta < n_cta && warp == 8) {
-            // ---- MMA issuer
-            constexpr uint32_t IS = pt_idesc<BF>(PT_BK, false), IO = pt_idesc<BF>(HD, true);
+        } else if (cta < n_cta && (warp == 8 || warp == 11)) {
+            // ---- MMA issuer of tile t
+            constexpr uint32_t IS = pt_idesc<BF>(64, false), IO = pt_idesc<BF>(HD, true);
+            const int t = warp == 8 ? 0 : 1;
             const uint32_t me = pt_elect();
-            uint32_t nq = 0, np[2] = {0, 0};
-            int ks = 0, kph = 0;  // ring stage and parity of step k's K tile; its V tile is the next
-            auto after = [&](int &st, int &ph) {
+            uint32_t nq = 0, np = 0;  // Q pairs used; parity of pready[t][h] in bit h
+            int st = 0, ph = 0;       // ring stage and parity of the next K or V tile
+            auto next = [&]() {
                 if (++st == NST) {
                     st = 0;
                     ph ^= 1;
                 }
             };
-            auto scores = [&](int t, int st) {  // S_t = Q_t K^T
-                const uint64_t a = pt_desc(pg_saddr(qbuf) + t * TB, 16), b = pt_desc(pg_saddr(ring) + st * TB, 16);
+            auto scores = [&](int h) {  // S_t,h = Q_t K_h^T
+                const uint64_t a = pt_desc(pg_saddr(qbuf) + t * TB, 16), b = pt_desc(pg_saddr(ring) + st * TB + h * 8192, 16);
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++) {
                     const uint32_t o = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-                    pt_mma_ss(me, tmem + t * 128, a + o, b + o, IS, k > 0);
+                    pt_mma_ss(me, tmem + t * 128 + h * 64, a + o, b + o, IS, k > 0);
                 }
-                pt_commit(me, &sh.sfull[t]);
+                pt_commit(me, &sh.sfull[t][h]);
             };
-            auto values = [&](int t, int st, bool first) {  // O_t += P_t V
-                const uint64_t b = pt_desc(pg_saddr(ring) + st * TB, 128 * 128);
+            auto values = [&](int h, int vst, bool first, bool last) {  // O_t += P_t,h V_h
+                const uint64_t b = pt_desc(pg_saddr(ring) + vst * TB + h * 8192, 128 * 128);
 #pragma unroll
-                for (int k = 0; k < PT_BK / 16; k++)
-                    pt_mma_ts(me, tmem + 256 + t * 128, tmem + t * 128 + 8 * k, b + k * (2048 >> 4), IO, !first || k > 0);
+                for (int k = 0; k < 4; k++)
+                    pt_mma_ts(me, tmem + 256 + t * 128, tmem + t * 128 + h * 64 + 8 * k, b + k * (2048 >> 4), IO, !first || k > 0);
+                pt_commit(me, &sh.pvdone[t]);
+                if (last) pt_commit(me, &sh.odone[t]);
             };
             for (uint32_t i = 0;; i++) {
                 bool ok = pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail);
@@ -388,49 +397,51 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 if (!ok) break;
                 const PtWork &w = sh.work[i & 1];
                 if (w.mode == PT_END) break;
-                const int b = w.b, e = w.e, ab0 = w.ab[0], ab1 = w.ab[1], ae0 = w.ae[0], ae1 = w.ae[1];
+                const int b = w.b, e = w.e, ab = w.ab[t], ae = w.ae[t];
+                const bool run = w.ae[0] > w.ab[0] || w.ae[1] > w.ab[1];
                 __syncwarp();
                 if (lane == 0) pg_arrive(&sh.wfree[i & 1]);
-                if (ae0 <= ab0 && ae1 <= ab1) continue;
-                auto on = [&](int t, int k) { return t == 0 ? k >= ab0 && k < ae0 : k >= ab1 && k < ae1; };
-                ok = pg_wait(&sh.qfull, nq & 1, &sh.fail) && pg_wait(&sh.kvfull[ks], kph, &sh.fail);
+                if (!run) continue;
+                auto on = [&](int j) { return j >= ab && j < ae; };
+                ok = pg_wait(&sh.qfull, nq & 1, &sh.fail) && pg_wait(&sh.kvfull[st], ph, &sh.fail);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 nq++;
                 pt_fence_after();
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-                    if (on(t, b)) scores(t, ks);
-                pt_commit(me, &sh.kvfree[ks]);
+                for (int h = 0; h < 2; h++)
+                    if (on(2 * b + h)) scores(h);
+                pt_commit(me, &sh.kvfree[st]);
                 if (e - b == 1) pt_commit(me, &sh.qfree);
+                next();
                 for (int k = b; k < e; k++) {
                     const bool more = k + 1 < e;
-                    int vs = ks, vph = kph;
-                    after(vs, vph);
-                    int ns = vs, nph = vph;  // the next step's K tile
-                    after(ns, nph);
-                    if (more) ok = pg_wait(&sh.kvfull[ns], nph, &sh.fail);
-                    ok = ok && pg_wait(&sh.kvfull[vs], vph, &sh.fail);
+                    const int vst = st;
+                    ok = pg_wait(&sh.kvfull[st], ph, &sh.fail);
+                    next();  // now the next step's K tile
 #pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        if (on(t, k)) {
-                            ok = ok && pg_wait(&sh.pready[t], np[t] & 1, &sh.fail);
+                    for (int h = 0; h < 2; h++) {
+                        if (on(2 * k + h)) {
+                            ok = ok && pg_wait(&sh.pready[t][h], np >> h & 1, &sh.fail);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
-                            np[t]++;
+                            np ^= 1u << h;
                             pt_fence_after();
-                            values(t, vs, k == (t == 0 ? ab0 : ab1));
-                            if (k + 1 == (t == 0 ? ae0 : ae1)) pt_commit(me, &sh.odone[t]);
+                            values(h, vst, 2 * k + h == ab, 2 * k + h + 1 == ae);
                         }
-                        if (t == 1) pt_commit(me, &sh.kvfree[vs]);
-                        if (more && on(t, k + 1)) scores(t, ns);
+                        if (h == 1) pt_commit(me, &sh.kvfree[vst]);
+                        if (more && h == 0) ok = ok && pg_wait(&sh.kvfull[st], ph, &sh.fail);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (more && on(2 * k + 2 + h)) scores(h);
                     }
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    if (more) pt_commit(me, &sh.kvfree[ns]);
-                    if (k + 2 == e) pt_commit(me, &sh.qfree);
-                    ks = ns;
-                    kph = nph;
+                    if (more) {
+                        pt_commit(me, &sh.kvfree[st]);
+                        if (k + 2 == e) pt_commit(me, &sh.qfree);
+                        next();
+                    }
                 }
                 if (!ok) break;
             }
@@ -444,7 +455,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
         const int t = warp >> 2, row = tid & 127;
         const uint32_t sa = tmem + t * 128 + ((uint32_t)(32 * (warp & 3)) << 16), oa = sa + 256;
         const uint64_t scale2 = pt_two(p.scale_log2, p.scale_log2);
-        uint32_t it = 0, ns = 0, no = 0, nj = 0;
+        uint32_t it = 0, ns = 0, npv = 0, no = 0, nj = 0;  // ns: parity of sfull[t][h] in bit h; npv: products of this tile
         for (uint32_t i = 0; cta < n_cta; i++) {
             if (!__all_sync(0xffffffffu, pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail))) break;
             const PtWork &w = sh.work[i & 1];
@@ -461,105 +472,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
             }
             const bool idle = 32 * (warp & 3) >= rows;  // no row of this warp exists: it only keeps step
             float m = -INFINITY, l = 0.f;
-            for (int k = ab; k < ae; k++) {
-                const int key0 = (w.kt0 + k) << PT_BK_SHIFT;
-                pg_wait(&sh.sfull[t], ns & 1, &sh.fail);
-                ns++;
+            auto await = [&](int j) {  // the scores of half step j are there
+                const int h = j & 1;
+                pg_wait(&sh.sfull[t][h], ns >> h & 1, &sh.fail);
+                ns ^= 1u << h;
                 pt_fence_after();
-                if (!idle) {
-                    float s[128];
-                    pt_ld32(s, sa);
-                    pt_ld32(s + 32, sa + 32);
-                    pt_wait_ld(s);
-                    pt_tie16(s + 16);
-                    pt_tie16(s + 32);
-                    pt_tie16(s + 48);
-                    pt_ld32(s + 64, sa + 64);
-                    pt_ld32(s + 96, sa + 96);
-                    float mx[4] = {s[0], s[1], s[2], s[3]};
-                    const bool masked = key0 < all_lo || key0 + PT_BK > all_hi;
+            };
+            auto fetch = [&](int j, float (&v)[64]) {
+                pt_ld32(v, sa + 64 * (j & 1));
+                pt_ld32(v + 32, sa + 64 * (j & 1) + 32);
+            };
+            // they have arrived in v: mask them, and the row's maximum among them
+            auto arrived = [&](int j, float (&v)[64]) -> float {
+                pt_wait_ld(v);
+                pt_tie16(v + 16);
+                pt_tie16(v + 32);
+                pt_tie16(v + 48);
+                const int key0 = (w.kt0 << PT_BK_SHIFT) + 64 * j;
+                if (key0 < all_lo || key0 + 64 > all_hi) {
                     const int ca = rlo - key0, cb = rhi - key0;  // columns [ca, cb) are seen
-                    if (masked) {
 #pragma unroll
-                        for (int c = 0; c < 64; c += 32) {
-                            const uint32_t keep = pt_below(cb - c) & ~pt_below(ca - c);
+                    for (int c = 0; c < 64; c += 32) {
+                        const uint32_t keep = pt_below(cb - c) & ~pt_below(ca - c);
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (!(keep >> j & 1)) s[c + j] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int c = 0; c < 4; c++) mx[c] = s[c];
+                        for (int n = 0; n < 32; n++)
+                            if (!(keep >> n & 1)) v[c + n] = -INFINITY;
                     }
-#pragma unroll
-                    for (int c = 4; c < 64; c += 8)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            mx[j] = c + 4 + j < 64 ? fmaxf(fmaxf(mx[j], s[c + j]), s[c + 4 + j]) : fmaxf(mx[j], s[c + j]);
-                    pt_wait_ld(s + 64);
-                    pt_tie16(s + 80);
-                    pt_tie16(s + 96);
-                    pt_tie16(s + 112);
-                    if (masked) {
-#pragma unroll
-                        for (int c = 64; c < 128; c += 32) {
-                            const uint32_t keep = pt_below(cb - c) & ~pt_below(ca - c);
-#pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (!(keep >> j & 1)) s[c + j] = -INFINITY;
-                        }
-                    }
-#pragma unroll
-                    for (int c = 64; c < 128; c += 8)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) mx[j] = fmaxf(fmaxf(mx[j], s[c + j]), s[c + 4 + j]);
-                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-                    const bool grow = mt > m + PT_GROWTH || (m == -INFINITY && mt > m);
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float mn = grow ? mt : m;
-                        const float f = grow ? pt_exp2(m - mn) : 1.f;
-                        m = mn;
-                        l *= f;
-                        if (k > ab) {
-#pragma unroll
-                            for (int c = 0; c < HD; c += 16) {
-                                float o[16];
-                                uint32_t x[16];
-                                pt_ld16(o, oa + c);
-                                pt_wait_ld(o);
-#pragma unroll
-                                for (int j = 0; j < 16; j++) x[j] = __float_as_uint(o[j] * f);
-                                pt_st16(oa + c, x);
-                            }
-                        }
-                    }
-                    const float nb = m == -INFINITY ? 0.f : -m;
-                    const uint64_t nb2 = pt_two(nb, nb);
-                    uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-                    for (int c = 0; c < 128; c += 32) {
-                        uint32_t x[16];
-#pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            float2 y = pt_both(pt_fma2(pt_two(s[c + 2 * j], s[c + 2 * j + 1]), scale2, nb2));
-                            if ((j & 3) < 4 - PT_POLY) {
-                                y.x = pt_exp2(y.x);
-                                y.y = pt_exp2(y.y);
-                            } else {
-                                y = pt_exp2_poly(y.x, y.y);
-                            }
-                            sum[j & 1] = pt_add2(sum[j & 1], pt_two(y.x, y.y));
-                            x[j] = pack2<BF>(y.x, y.y);
-                        }
-                        pt_st16(sa + c / 2, x);
-                    }
-                    const float2 l2 = pt_both(pt_add2(sum[0], sum[1]));
-                    l += l2.x + l2.y;
                 }
-                if ((key0 < w.lo || key0 + PT_BK > w.hi) && (t == 0 || k < w.ab[0] || k >= w.ae[0])) {
+                float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                for (int c = 4; c < 60; c += 8)
+#pragma unroll
+                    for (int n = 0; n < 4; n++) mx[n] = fmaxf(fmaxf(mx[n], v[c + n]), v[c + 4 + n]);
+                return fmaxf(fmaxf(fmaxf(mx[0], v[60]), fmaxf(mx[1], v[61])), fmaxf(fmaxf(mx[2], v[62]), fmaxf(mx[3], v[63]))) *
+                       p.scale_log2;
+            };
+            // probabilities of half step j are written: hand them over
+            auto hand_over = [&](int j) {
+                const int h = j & 1, tile0 = (w.kt0 + (j >> 1)) << PT_BK_SHIFT;
+                npv++;
+                if ((h == 0 || j == ab) && (tile0 < w.lo || tile0 + PT_BK > w.hi) && (t == 0 || j < w.ab[0] || j >= w.ae[0])) {
                     // values no row of the unit sees may hold anything: weight 0 must meet 0 there
-                    const uint32_t vi = it + 2 * (k - w.b) + 1;
+                    const uint32_t vi = it + 2 * ((j >> 1) - w.b) + 1;
                     pg_wait(&sh.kvfull[vi % NST], vi / NST & 1, &sh.fail);
-                    if (key0 + row < w.lo || key0 + row >= w.hi)
+                    if (tile0 + row < w.lo || tile0 + row >= w.hi)
 #pragma unroll 1
                         for (int c = 0; c < 8 * HALVES; c++)  // pieces rotated by the row: eight rows on eight banks
                             *reinterpret_cast<uint4 *>(ring + (vi % NST) * TB + (c >> 3) * (128 * 128) + row * 128 +
@@ -569,14 +525,71 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 pt_wait_st();
                 pt_fence_before();
                 __syncwarp();
-                if (lane == 0) pg_arrive(&sh.pready[t]);
+                if (lane == 0) pg_arrive(&sh.pready[t][h]);
+            };
+            auto half_step = [&](int j) {
+                float v[64];
+                await(j);
+                fetch(j, v);
+                const float mt = arrived(j, v);
+                const bool grow = mt > m + PT_GROWTH || (m == -INFINITY && mt > m);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float mn = grow ? mt : m;
+                    const float f = grow ? pt_exp2(m - mn) : 1.f;
+                    m = mn;
+                    l *= f;
+                    if (j > ab) {
+                        pg_wait(&sh.pvdone[t], (npv - 1) & 1, &sh.fail);  // the half before is in O (the one before
+                        pt_fence_after();                                 // that had finished when v's scores did)
+#pragma unroll
+                        for (int c = 0; c < HD; c += 16) {
+                            float o[16];
+                            uint32_t x[16];
+                            pt_ld16(o, oa + c);
+                            pt_wait_ld(o);
+#pragma unroll
+                            for (int n = 0; n < 16; n++) x[n] = __float_as_uint(o[n] * f);
+                            pt_st16(oa + c, x);
+                        }
+                    }
+                }
+                const float nb = m == -INFINITY ? 0.f : -m;
+                const uint64_t nb2 = pt_two(nb, nb);
+                uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < 64; c += 32) {
+                    uint32_t x[16];
+#pragma unroll
+                    for (int n = 0; n < 16; n++) {
+                        float2 y = pt_both(pt_fma2(pt_two(v[c + 2 * n], v[c + 2 * n + 1]), scale2, nb2));
+                        if ((n & 3) < 4 - PT_POLY) {
+                            y.x = pt_exp2(y.x);
+                            y.y = pt_exp2(y.y);
+                        } else {
+                            y = pt_exp2_poly(y.x, y.y);
+                        }
+                        sum[n & 1] = pt_add2(sum[n & 1], pt_two(y.x, y.y));
+                        x[n] = pack2<BF>(y.x, y.y);
+                    }
+                    pt_st16(sa + 64 * (j & 1) + c / 2, x);
+                }
+                const float2 l2 = pt_both(pt_add2(sum[0], sum[1]));
+                l += l2.x + l2.y;
+                hand_over(j);
+            };
+            if (idle) {
+                for (int j = ab; j < ae; j++) {
+                    await(j);
+                    hand_over(j);
+                }
+            } else {
+                for (int j = ab; j < ae; j++) half_step(j);
             }
             // ---- the unit's (or piece's) output
             if (w.ae[0] > w.ab[0] || w.ae[1] > w.ab[1]) it += 2 * (w.e - w.b);
             const bool did = ae > ab;
             if (did) {
-                pg_wait(&sh.odone[t], no & 1, &sh.fail);
-                no++;
+                pg_wait(&sh.odone[t], no++ & 1, &sh.fail);
                 pt_fence_after();
             }
             const int tok = fdiv(row0 + row, p.by_group), head = w.g * p.group + row0 + row - tok * p.group;
