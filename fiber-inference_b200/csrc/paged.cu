@@ -166,6 +166,9 @@ cudaError_t launch_append(const AppendParams &p, int hd, cudaStream_t st) {
 constexpr size_t WS_TICKETS = 256, WS_PARTS = WS_TICKETS + 4096;
 constexpr int WS_MAX_CTAS = 1024;
 
+// {unit, half, full, share}
+constexpr AttnCost PR_COST = {3, 1, 1, 1}, PT_COST = {4, 3, 4, 4};
+
 struct AttnShape {
     bool tile;        // tile kernel, else row kernel
     int n_cta, rows;  // CTAs of a launch, rows of a unit's state
@@ -208,9 +211,9 @@ int check_attn(const char *fn, const fiber_kv_view_t *kv, const fiber_ragged_t *
     if (b->n_tokens && b->max_q < 1) return fail(FIBER_EARG, "%s: max_q %d", fn, b->max_q);
     if (n_heads <= 0 || n_heads % kv->n_kv_heads || n_heads / kv->n_kv_heads > 128)
         return fail(FIBER_EARG, "%s: %d query heads over %d KV heads", fn, n_heads, kv->n_kv_heads);
-    // steps of a launch are counted in 32 bits
+    // the cost of a launch is counted in 32 bits
     const double rows = (double)b->n_tokens * (n_heads / kv->n_kv_heads) / PR_ROWS + b->n_seqs;
-    if (rows * kv->n_kv_heads * ((double)kv->max_pages * kv->page_size / PR_BK + 2) > 4e9)
+    if (rows * kv->n_kv_heads * ((double)kv->max_pages * kv->page_size / PR_BK + 8) > 1e9)
         return fail(FIBER_EARG, "%s: batch too large (%d tokens over %d positions)", fn, b->n_tokens,
                     kv->max_pages * kv->page_size);
     return FIBER_OK;
@@ -322,6 +325,7 @@ extern "C" int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t 
     p.by_group = make_div((uint32_t)p.group);
     p.by_ru = make_div(shape.tile ? 2u * pt_tile_rows(p.group) : (unsigned)PR_ROWS);
     p.window = window;
+    p.cost = shape.tile ? PT_COST : PR_COST;
     p.scale = scale;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
     uint8_t *ws = (uint8_t *)d_ws;

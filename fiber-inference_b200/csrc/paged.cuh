@@ -161,6 +161,12 @@ FDEV void pg_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "
 
 // ---- attention -----------------------------------------------------------------------------
 
+// What the division of the work counts: a unit costs `unit` plus `half` (up to half of its
+// rows in use) or `full` per tile of keys; a CTA's share is at least `share`.
+struct AttnCost {
+    int unit, half, full, share;
+};
+
 struct AttnPagedParams {
     CUtensorMap kmap, vmap;  // (head_dim, page_size, n_kv, n_pages); 128-byte swizzle
     CUtensorMap qmap;        // tile kernel: (head_dim, n_heads, n_tokens)
@@ -173,6 +179,7 @@ struct AttnPagedParams {
     FastDiv by_group, by_ru;  // by_ru: rows of a unit
     int window;
     float scale, scale_log2;  // scale * log2(e): scores in powers of two
+    AttnCost cost;
     int *status;              // workspace: set to 1 when a wait gave up
     unsigned int *tickets;    // one per CTA, zero between calls
     float *part_ml;           // [2 * n_cta][rows][2]: running maximum (powers of two) and sum
@@ -183,11 +190,12 @@ constexpr int PG_MAX_SEQS = 128;  // sequences of one launch; larger batches tak
 
 // How a launch's work is divided. The rows (token, head of the group) of a sequence and KV
 // head are cut into units of RU rows; a unit takes one step per tile of BK keys that any
-// of its rows sees (at least one, so rows that see nothing are written too). All steps in
-// the order (sequence, KV head, unit, tile) are numbered 0 .. T - 1 and CTA c of n takes
-// steps [c T / n, (c + 1) T / n): equal shares whatever the lengths. A unit that is
-// cut between CTAs leaves one softmax state per CTA; the last CTA to finish (ticket)
-// joins them in CTA order, so the result does not depend on the timing.
+// of its rows sees (at least one, so rows that see nothing are written too). The costs of
+// all units in the order (sequence, KV head, unit) are laid end to end, 0 .. T, and CTA c
+// of n takes the steps whose places lie in [c T / n, (c + 1) T / n): equal shares whatever
+// the lengths. A unit that is cut between CTAs leaves one softmax state per CTA; the last
+// CTA to finish (ticket) joins them in CTA order, so the result does not depend on the
+// timing.
 struct AttnPlan {
     uint32_t prefix[PG_MAX_SEQS + 1];
     int4 seq[PG_MAX_SEQS];  // q0, nq, kv, slot
@@ -198,7 +206,8 @@ struct AttnUnit {
     int q0, nq, kv, slot;  // of the sequence
     int row0, rows;        // rows of the unit: row0 .. row0 + rows - 1 of nq * group
     int lo, hi;            // positions any row of the unit sees
-    uint32_t u0, steps;    // number of its first step, and its steps
+    uint32_t u0, cost;     // where it starts, and what it costs
+    int steps, per;        // its steps, and what one costs
 };
 
 // Positions that the rows [row0, row0 + rows) see together.
@@ -208,12 +217,16 @@ FDEV void attn_span(int nq, int kv, const AttnPagedParams &p, int row0, int rows
     lo = p.window > 0 ? max(0, p0 + t0 - p.window + 1) : 0;
 }
 
-FDEV uint32_t attn_steps(int nq, int kv, const AttnPagedParams &p, int ru, int bk_shift, int i) {
-    const int row0 = i * ru;
+FDEV int attn_steps(int lo, int hi, int bk_shift) {
+    return max(1, hi > lo ? ((hi + (1 << bk_shift) - 1) >> bk_shift) - (lo >> bk_shift) : 0);
+}
+FDEV int attn_per(const AttnPagedParams &p, int rows, int ru) { return 2 * rows > ru ? p.cost.full : p.cost.half; }
+
+FDEV uint32_t attn_unit_cost(int nq, int kv, const AttnPagedParams &p, int ru, int bk_shift, int i) {
+    const int row0 = i * ru, rows = min(ru, nq * p.group - row0);
     int lo, hi;
-    attn_span(nq, kv, p, row0, min(ru, nq * p.group - row0), lo, hi);
-    const int tiles = ((hi + (1 << bk_shift) - 1) >> bk_shift) - (lo >> bk_shift);
-    return (uint32_t)max(1, hi > lo ? tiles : 0);
+    attn_span(nq, kv, p, row0, rows, lo, hi);
+    return (uint32_t)(p.cost.unit + attn_per(p, rows, ru) * attn_steps(lo, hi, bk_shift));
 }
 
 // Fill the plan (all threads of the CTA; ends with a barrier) and return T.
@@ -228,7 +241,7 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
         const int nu = fdiv(q.nq * p.group + ru - 1, p.by_ru);
         uint32_t sum = 0;
         if (nu <= SHORT)
-            for (int i = 0; i < nu; i++) sum += attn_steps(q.nq, q.kv, p, ru, bk_shift, i);
+            for (int i = 0; i < nu; i++) sum += attn_unit_cost(q.nq, q.kv, p, ru, bk_shift, i);
         pl.prefix[s + 1] = sum;
     }
     if (tid == 0) pl.prefix[0] = 0;
@@ -238,7 +251,7 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
         const int nu = fdiv(q.y * p.group + ru - 1, p.by_ru);
         if (nu <= SHORT) continue;
         uint32_t sum = 0;
-        for (int i = lane; i < nu; i += 32) sum += attn_steps(q.y, q.z, p, ru, bk_shift, i);
+        for (int i = lane; i < nu; i += 32) sum += attn_unit_cost(q.y, q.z, p, ru, bk_shift, i);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) pl.prefix[s + 1] = sum;
@@ -271,10 +284,12 @@ FDEV void attn_unit_fill(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
     u.row0 = u.i * ru;
     u.rows = min(ru, u.nq * p.group - u.row0);
     attn_span(u.nq, u.kv, p, u.row0, u.rows, u.lo, u.hi);
-    u.steps = attn_steps(u.nq, u.kv, p, ru, bk_shift, u.i);
+    u.steps = attn_steps(u.lo, u.hi, bk_shift);
+    u.per = attn_per(p, u.rows, ru);
+    u.cost = (uint32_t)(p.cost.unit + u.per * u.steps);
 }
 
-// The unit that holds step x; all lanes of a warp together.
+// The unit that holds place x; all lanes of a warp together.
 FDEV void attn_unit_find(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift, uint32_t x) {
     const int lane = threadIdx.x & 31;
     int a = 0, b = p.b.n_seqs;  // prefix[a] <= x < prefix[b]
@@ -292,7 +307,7 @@ FDEV void attn_unit_find(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
     const int4 q = pl.seq[a];
     const int nu = fdiv(q.y * p.group + ru - 1, p.by_ru);
     for (int i0 = 0;; i0 += 32) {
-        uint32_t n = i0 + lane < nu ? attn_steps(q.y, q.z, p, ru, bk_shift, i0 + lane) : 0, sum = n;
+        uint32_t n = i0 + lane < nu ? attn_unit_cost(q.y, q.z, p, ru, bk_shift, i0 + lane) : 0, sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t t = __shfl_up_sync(0xffffffffu, sum, o);
@@ -313,7 +328,7 @@ FDEV void attn_unit_find(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
 
 // The unit after u (the caller knows there is one).
 FDEV void attn_unit_next(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift) {
-    u.u0 += u.steps;
+    u.u0 += u.cost;
     u.i++;
     if (u.i * ru >= u.nq * p.group) {
         u.i = 0;
@@ -327,10 +342,23 @@ FDEV void attn_unit_next(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
     attn_unit_fill(u, pl, p, ru, bk_shift);
 }
 
-// First step of CTA c's share, and the CTA that holds step x.
+// CTAs of a launch, the start of CTA c's share, and the CTA whose share holds place x.
+FDEV int attn_ctas(const AttnPagedParams &p, uint32_t total) {
+    return total == 0 ? 0 : min((int)gridDim.x, max(1, (int)(total / (uint32_t)p.cost.share)));
+}
 FDEV uint32_t attn_share(uint32_t total, int n_cta, int c) { return (uint32_t)((unsigned long long)total * c / n_cta); }
 FDEV int attn_owner(uint32_t total, int n_cta, uint32_t x) {
     return (int)((((unsigned long long)x + 1) * n_cta - 1) / total);
+}
+// Step k of a unit lies at the place u0 + unit + k per. A share spans at least one step's
+// cost, so every CTA between a cut unit's first and last has a piece of it.
+FDEV uint32_t attn_place(const AttnUnit &u, const AttnPagedParams &p, int k) {
+    return u.u0 + (uint32_t)(p.cost.unit + k * u.per);
+}
+// The first step of the unit at or after place x.
+FDEV int attn_step_at(const AttnUnit &u, const AttnPagedParams &p, uint32_t x) {
+    const int d = (int)(x - u.u0) - p.cost.unit;
+    return d <= 0 ? 0 : min(u.steps, u.per == 1 ? d : (d + u.per - 1) / u.per);
 }
 
 // One row from the definition, by one warp: only the positions the row sees are read, so

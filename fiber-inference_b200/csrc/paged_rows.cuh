@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
     pdl_trigger();
     pdl_wait();
     const uint32_t total = attn_plan_build<PR_THREADS>(sh.plan, p, PR_ROWS, PR_BK_SHIFT);
-    const int n_cta = min((int)gridDim.x, (int)min(total, 0x7fffffffu)), cta = blockIdx.x;
+    const int n_cta = attn_ctas(p, total), cta = blockIdx.x;
     if (cta >= n_cta) return;
     const uint32_t x0 = attn_share(total, n_cta, cta), x1 = attn_share(total, n_cta, cta + 1);
     AttnUnit u;
@@ -105,13 +105,13 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         const uint32_t dst0 = (is_v ? SB / 2 : 0) + half * (PR_BK * 128) + rb * box_rows * 128;
         uint32_t it = 0;
         bool ok = true;
-        for (uint32_t x = x0;;) {
-            const uint32_t b = x - u.u0, e = min(x1 - u.u0, u.steps);
+        for (;;) {
+            const int b = u.u0 < x0 ? attn_step_at(u, p, x0) : 0, e = u.u0 + u.cost > x1 ? attn_step_at(u, p, x1) : u.steps;
             if (u.hi > u.lo) {
                 const int32_t *tab = p.kv.table + (long long)u.slot * p.kv.max_pages;
                 const int used = (u.hi + (1 << p.kv.page_shift) - 1) >> p.kv.page_shift;
-                for (uint32_t k = b; k < e; k++, it++) {
-                    const int key = (((u.lo >> PR_BK_SHIFT) + (int)k) << PR_BK_SHIFT) + rb * box_rows;
+                for (int k = b; k < e; k++, it++) {
+                    const int key = (((u.lo >> PR_BK_SHIFT) + k) << PR_BK_SHIFT) + rb * box_rows;
                     const int lp = key >> p.kv.page_shift;
                     int page = p.kv.n_pages;  // outside the tensor: reads as zeros
                     if (lane < n_box && lp < used) page = tab[lp];
@@ -126,8 +126,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                                 key & ((1 << p.kv.page_shift) - 1), u.g, page, &sh.full[st]);
                 }
             }
-            x = u.u0 + e;
-            if (!ok || x >= x1) break;
+            if (!ok || u.u0 + u.cost >= x1) break;
             attn_unit_next(u, sh.plan, p, PR_ROWS, PR_BK_SHIFT);
         }
         // every copy has landed before the CTA exits
@@ -141,8 +140,8 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
     // ---- consumers: warp w takes keys 16 w .. 16 w + 15 of each tile
     const int g8 = lane >> 2, t4 = lane & 3;
     uint32_t it = 0;
-    for (uint32_t x = x0;;) {
-        const uint32_t b = x - u.u0, e = min(x1 - u.u0, u.steps);
+    for (;;) {
+        const int b = u.u0 < x0 ? attn_step_at(u, p, x0) : 0, e = u.u0 + u.cost > x1 ? attn_step_at(u, p, x1) : u.steps;
         const bool whole = b == 0 && e == u.steps, any = u.hi > u.lo;
         const int p0 = u.kv - u.nq;
         // query fragments, and the positions that rows g8 and g8 + 8 see
@@ -168,12 +167,12 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         const int all_hi = max(0, p0 + fdiv(u.row0, p.by_group) + 1);
         const int all_lo = p.window > 0 ? max(0, p0 + fdiv(u.row0 + u.rows - 1, p.by_group) - p.window + 1) : 0;
         int st = 0;
-        if (any) {
-            for (uint32_t k = b; k < e; k++, it++) {
+        if (any && b < e) {
+            for (int k = b; k < e; k++, it++) {
                 st = it % NST;
                 pg_wait(&sh.full[st], (it / NST) & 1, &sh.fail);  // after a timeout: runs through, status says so
                 uint8_t *kt = ring + st * SB, *vt = kt + SB / 2;
-                const int key0 = (((u.lo >> PR_BK_SHIFT) + (int)k) << PR_BK_SHIFT) + 16 * warp;
+                const int key0 = (((u.lo >> PR_BK_SHIFT) + k) << PR_BK_SHIFT) + 16 * warp;
                 const bool edge = key0 < all_lo || key0 + 16 > all_hi;
                 if (edge && (key0 < u.lo || key0 + 16 > u.hi)) {
                     // values no row sees may hold anything: weight 0 must meet 0 there
@@ -300,7 +299,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
             if (lane == 0) pg_arrive(&sh.empty[st]);
             if (!whole) {
                 // ---- join the CTAs' states of this unit
-                const int ca = attn_owner(total, n_cta, u.u0), cb = attn_owner(total, n_cta, u.u0 + u.steps - 1);
+                const int ca = attn_owner(total, n_cta, attn_place(u, p, 0)), cb = attn_owner(total, n_cta, attn_place(u, p, u.steps - 1));
                 if (tid == 0) {
                     sh.last = atomicAdd(&p.tickets[ca], 1u) == (unsigned)(cb - ca);
                     if (sh.last) p.tickets[ca] = 0u;
@@ -368,7 +367,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                 if (tid == 0) sh.bad = 0;
             }
             pr_bar();  // sh.ml and sh.bad are reused by the next unit
-        } else {
+        } else if (b < e) {  // no row of the unit sees a key
             for (int i = tid; i < u.rows * C4; i += 32 * PR_WARPS) {
                 const int r = i / C4, c4 = i % C4;
                 const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
@@ -376,8 +375,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                     make_uint2(0u, 0u);
             }
         }
-        x = u.u0 + e;
-        if (x >= x1) break;
+        if (u.u0 + u.cost >= x1) break;
         attn_unit_next(u, sh.plan, p, PR_ROWS, PR_BK_SHIFT);
     }
     if (lane == 0 && sh.fail) *p.status = 1;

@@ -249,24 +249,29 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
     pt_fence_after();
     constexpr uint32_t tmem = 0;  // all 512 columns
     if (sh.tmem != tmem && tid == 0) *p.status = 2;
-    const int n_cta = min((int)gridDim.x, (int)min(total, 0x7fffffffu)), cta = blockIdx.x;
+    const int n_cta = attn_ctas(p, total), cta = blockIdx.x;
 
     // 384 threads at 168 registers: the softmax warpgroups take 224 each, the third keeps 56
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (cta < n_cta && warp == 10) {
             // ---- scheduler
-            const uint32_t x1 = attn_share(total, n_cta, cta + 1);
-            uint32_t x = attn_share(total, n_cta, cta);
+            const uint32_t x0 = attn_share(total, n_cta, cta), x1 = attn_share(total, n_cta, cta + 1);
             AttnUnit u;
-            attn_unit_find(u, sh.plan, p, ru, PT_BK_SHIFT, x);
-            for (uint32_t i = 0;; i++) {
+            attn_unit_find(u, sh.plan, p, ru, PT_BK_SHIFT, x0);
+            bool end = false;
+            for (uint32_t i = 0;;) {
+                const int b = u.u0 < x0 ? attn_step_at(u, p, x0) : 0, e = u.u0 + u.cost > x1 ? attn_step_at(u, p, x1) : u.steps;
+                const int kt0 = u.lo >> PT_BK_SHIFT;
+                if (!end && b >= e) {  // none of this unit's steps
+                    end = u.u0 + u.cost >= x1;
+                    if (!end) attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+                    continue;
+                }
                 bool ok = i < 2 || pg_wait(&sh.wfree[i & 1], ((i >> 1) - 1) & 1, &sh.fail);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 PtWork &w = sh.work[i & 1];
-                const bool end = x >= x1;
-                const int b = (int)(x - u.u0), e = (int)min(x1 - u.u0, u.steps), kt0 = u.lo >> PT_BK_SHIFT;
                 if (lane < 2 && !end) {  // lane t: tile t
                     const int rows = lane == 0 ? min(rt, u.rows) : max(0, u.rows - rt);
                     int lo = 0, hi = 0, ab = 0, ae = 0;
@@ -280,7 +285,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                     w.ae[lane] = ae;
                 }
                 if (lane == 0) {
-                    w.mode = end ? PT_END : (b == 0 && e == (int)u.steps ? PT_WHOLE : PT_PIECE);
+                    w.mode = end ? PT_END : (b == 0 && e == u.steps ? PT_WHOLE : PT_PIECE);
                     if (!end) {
                         w.q0 = u.q0;
                         w.slot = u.slot;
@@ -293,15 +298,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                         w.b = b;
                         w.e = e;
                         w.slot_of = 2 * cta + (b > 0 ? 0 : 1);
-                        w.ca = attn_owner(total, n_cta, u.u0);
-                        w.cb = attn_owner(total, n_cta, u.u0 + u.steps - 1);
+                        w.ca = attn_owner(total, n_cta, attn_place(u, p, 0));
+                        w.cb = attn_owner(total, n_cta, attn_place(u, p, u.steps - 1));
                     }
                 }
                 __syncwarp();
                 if (lane == 0) pg_arrive(&sh.wfull[i & 1]);
                 if (end) break;
-                x = u.u0 + (uint32_t)e;
-                if (x < x1) attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
+                i++;
+                end = u.u0 + u.cost >= x1;
+                if (!end) attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
             }
         } else if (cta < n_cta && warp == 9) {
             // ---- producer: lane b issues box b of a K or V tile
