@@ -166,8 +166,8 @@ cudaError_t launch_append(const AppendParams &p, int hd, cudaStream_t st) {
 constexpr size_t WS_TICKETS = 256, WS_PARTS = WS_TICKETS + 4096;
 constexpr int WS_MAX_CTAS = 1024;
 
-// {unit, half, full, share}
-constexpr AttnCost PR_COST = {3, 1, 1, 1}, PT_COST = {4, 3, 4, 4};
+// {unit, half, full, snap, share, root}
+constexpr AttnCost PR_COST = {3, 1, 1, 8, 1, 0.8f}, PT_COST = {4, 3, 4, 4, 4, 1.0f};
 
 struct AttnShape {
     bool tile;        // tile kernel, else row kernel

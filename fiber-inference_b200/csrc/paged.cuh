@@ -157,14 +157,26 @@ FDEV void pg_tma3(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, 
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(pg_saddr(bar))
         : "memory");
 }
+FDEV void pg_prefetch_map(const CUtensorMap *map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+FDEV unsigned pg_ticket(unsigned *t) {  // orders this CTA's writes before, the others' after it
+    unsigned v;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(v) : "l"(t) : "memory");
+    return v;
+}
 FDEV void pg_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- attention -----------------------------------------------------------------------------
 
 // What the division of the work counts: a unit costs `unit` plus `half` (up to half of its
-// rows in use) or `full` per tile of keys; a CTA's share is at least `share`.
+// rows in use) or `full` per tile of keys. A unit of up to `snap` steps is not cut. A CTA's
+// share is at least `share`, and at least `root` times the root of the longest unit's cost
+// where that is known: with shares of x a unit costs x steps in a row and then a join of
+// cost / x states, which is least at x ~ sqrt(cost).
 struct AttnCost {
-    int unit, half, full, share;
+    int unit, half, full, snap, share;
+    float root;
 };
 
 struct AttnPagedParams {
@@ -207,7 +219,7 @@ struct AttnUnit {
     int row0, rows;        // rows of the unit: row0 .. row0 + rows - 1 of nq * group
     int lo, hi;            // positions any row of the unit sees
     uint32_t u0, cost;     // where it starts, and what it costs
-    int steps, per;        // its steps, and what one costs
+    int steps, per;        // its steps, and what one costs (0: all of them lie where it starts)
 };
 
 // Positions that the rows [row0, row0 + rows) see together.
@@ -229,31 +241,72 @@ FDEV uint32_t attn_unit_cost(int nq, int kv, const AttnPagedParams &p, int ru, i
     return (uint32_t)(p.cost.unit + attn_per(p, rows, ru) * attn_steps(lo, hi, bk_shift));
 }
 
-// Fill the plan (all threads of the CTA; ends with a barrier) and return T.
+// What the units of a sequence cost together, per KV head; all lanes of a warp.
+FDEV uint32_t attn_seq_cost(int nq, int kv, const AttnPagedParams &p, int ru, int bk_shift, int lane) {
+    const int nu = fdiv(nq * p.group + ru - 1, p.by_ru);
+    uint32_t sum = 0;
+    for (int i = lane; i < nu; i += 32) sum += attn_unit_cost(nq, kv, p, ru, bk_shift, i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
+// Fill the plan and return T; `longest`: the largest unit's cost, or 0. Up to 32 sequences each warp does it for itself (all write
+// the same), without a barrier: one round trip for the lengths. More are shared among the
+// CTA's threads.
 template <int THREADS>
-FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift) {
+FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift, uint32_t &longest) {
     const int tid = threadIdx.x, lane = tid & 31, ns = p.b.n_seqs;
-    constexpr int SHORT = 8;  // sequences of more units are summed by whole warps
+    constexpr int SHORT = 4;  // sequences of more units are summed by whole warps
+    auto load = [&](int s) {
+        return make_seq(p.b, p.kv, p.b.q_start[s], p.b.q_start[s + 1], p.b.kv_len[s], p.b.slot ? p.b.slot[s] : p.b.slot0 + s);
+    };
+    auto few = [&](const SeqInfo &q, int nu) {
+        uint32_t sum = 0;
+        for (int i = 0; i < nu; i++) sum += attn_unit_cost(q.nq, q.kv, p, ru, bk_shift, i);
+        return sum;
+    };
+    auto scan = [&](uint32_t v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += t;
+        }
+        return v;
+    };
+    if (ns <= 32) {
+        SeqInfo q = {0, 0, 0, 0};
+        if (lane < ns) q = load(lane);
+        const int nu = fdiv(q.nq * p.group + ru - 1, p.by_ru);
+        uint32_t sum = nu <= SHORT ? few(q, nu) : 0;
+        for (unsigned big = __ballot_sync(0xffffffffu, nu > SHORT); big; big &= big - 1) {
+            const int s = __ffs(big) - 1;
+            const uint32_t v = attn_seq_cost(__shfl_sync(0xffffffffu, q.nq, s), __shfl_sync(0xffffffffu, q.kv, s), p, ru, bk_shift, lane);
+            if (lane == s) sum = v;
+        }
+        longest = __reduce_max_sync(0xffffffffu, nu > 0 ? attn_unit_cost(q.nq, q.kv, p, ru, bk_shift, nu - 1) : 0u);
+        sum = scan(sum * (uint32_t)p.kv.n_kv);
+        if (lane < ns) {
+            pl.seq[lane] = make_int4(q.q0, q.nq, q.kv, q.slot);
+            pl.prefix[lane + 1] = sum;
+        }
+        if (lane == 0) pl.prefix[0] = 0;
+        __syncwarp();
+        return __shfl_sync(0xffffffffu, sum, 31);
+    }
+    longest = 0;
     for (int s = tid; s < ns; s += THREADS) {
-        const SeqInfo q = make_seq(p.b, p.kv, p.b.q_start[s], p.b.q_start[s + 1], p.b.kv_len[s],
-                                   p.b.slot ? p.b.slot[s] : p.b.slot0 + s);
+        const SeqInfo q = load(s);
         pl.seq[s] = make_int4(q.q0, q.nq, q.kv, q.slot);
         const int nu = fdiv(q.nq * p.group + ru - 1, p.by_ru);
-        uint32_t sum = 0;
-        if (nu <= SHORT)
-            for (int i = 0; i < nu; i++) sum += attn_unit_cost(q.nq, q.kv, p, ru, bk_shift, i);
-        pl.prefix[s + 1] = sum;
+        pl.prefix[s + 1] = nu <= SHORT ? few(q, nu) : 0;
     }
     if (tid == 0) pl.prefix[0] = 0;
     __syncthreads();
     for (int s = tid >> 5; s < ns; s += THREADS / 32) {
         const int4 q = pl.seq[s];
-        const int nu = fdiv(q.y * p.group + ru - 1, p.by_ru);
-        if (nu <= SHORT) continue;
-        uint32_t sum = 0;
-        for (int i = lane; i < nu; i += 32) sum += attn_unit_cost(q.y, q.z, p, ru, bk_shift, i);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (fdiv(q.y * p.group + ru - 1, p.by_ru) <= SHORT) continue;
+        const uint32_t sum = attn_seq_cost(q.y, q.z, p, ru, bk_shift, lane);
         if (lane == 0) pl.prefix[s + 1] = sum;
     }
     __syncthreads();
@@ -261,12 +314,8 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
         uint32_t base = 0;
         for (int s0 = 0; s0 < ns; s0 += 32) {
             const int s = s0 + lane;
-            uint32_t v = s < ns ? pl.prefix[s + 1] * (uint32_t)p.kv.n_kv : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t t = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += t;
-            }
+            const uint32_t v = scan(s < ns ? pl.prefix[s + 1] * (uint32_t)p.kv.n_kv : 0);
+            __syncwarp();
             if (s < ns) pl.prefix[s + 1] = base + v;
             base += __shfl_sync(0xffffffffu, v, 31);
         }
@@ -287,6 +336,7 @@ FDEV void attn_unit_fill(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
     u.steps = attn_steps(u.lo, u.hi, bk_shift);
     u.per = attn_per(p, u.rows, ru);
     u.cost = (uint32_t)(p.cost.unit + u.per * u.steps);
+    if (u.steps <= p.cost.snap) u.per = 0;
 }
 
 // The unit that holds place x; all lanes of a warp together.
@@ -343,8 +393,9 @@ FDEV void attn_unit_next(AttnUnit &u, const AttnPlan &pl, const AttnPagedParams 
 }
 
 // CTAs of a launch, the start of CTA c's share, and the CTA whose share holds place x.
-FDEV int attn_ctas(const AttnPagedParams &p, uint32_t total) {
-    return total == 0 ? 0 : min((int)gridDim.x, max(1, (int)(total / (uint32_t)p.cost.share)));
+FDEV int attn_ctas(const AttnPagedParams &p, uint32_t total, uint32_t longest) {
+    const uint32_t share = max((uint32_t)p.cost.share, (uint32_t)(p.cost.root * sqrtf((float)longest)));
+    return total == 0 ? 0 : (int)min(gridDim.x, max(1u, total / share));
 }
 FDEV uint32_t attn_share(uint32_t total, int n_cta, int c) { return (uint32_t)((unsigned long long)total * c / n_cta); }
 FDEV int attn_owner(uint32_t total, int n_cta, uint32_t x) {
@@ -353,10 +404,11 @@ FDEV int attn_owner(uint32_t total, int n_cta, uint32_t x) {
 // Step k of a unit lies at the place u0 + unit + k per. A share spans at least one step's
 // cost, so every CTA between a cut unit's first and last has a piece of it.
 FDEV uint32_t attn_place(const AttnUnit &u, const AttnPagedParams &p, int k) {
-    return u.u0 + (uint32_t)(p.cost.unit + k * u.per);
+    return u.u0 + (u.per ? (uint32_t)(p.cost.unit + k * u.per) : 0u);
 }
 // The first step of the unit at or after place x.
 FDEV int attn_step_at(const AttnUnit &u, const AttnPagedParams &p, uint32_t x) {
+    if (u.per == 0) return x > u.u0 ? u.steps : 0;
     const int d = (int)(x - u.u0) - p.cost.unit;
     return d <= 0 ? 0 : min(u.steps, u.per == 1 ? d : (d + u.per - 1) / u.per);
 }

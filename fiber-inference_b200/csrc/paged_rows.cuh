@@ -28,7 +28,6 @@ struct PrShared {
     AttnPlan plan;
     uint64_t full[8], empty[8];
     float ml[PR_WARPS][PR_ROWS][2];
-    float row_m[PR_ROWS], row_l[PR_ROWS];
     unsigned bad;  // rows whose result is not finite
     int last;
     int fail;
@@ -86,10 +85,16 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         sh.fail = 0;
         sh.bad = 0;
     }
+    if (tid == 32 * PR_WARPS) {
+        pg_prefetch_map(&p.kmap);
+        pg_prefetch_map(&p.vmap);
+    }
+    __syncthreads();
     pdl_trigger();
     pdl_wait();
-    const uint32_t total = attn_plan_build<PR_THREADS>(sh.plan, p, PR_ROWS, PR_BK_SHIFT);
-    const int n_cta = attn_ctas(p, total), cta = blockIdx.x;
+    uint32_t longest;
+    const uint32_t total = attn_plan_build<PR_THREADS>(sh.plan, p, PR_ROWS, PR_BK_SHIFT, longest);
+    const int n_cta = attn_ctas(p, total, longest), cta = blockIdx.x;
     if (cta >= n_cta) return;
     const uint32_t x0 = attn_share(total, n_cta, cta), x1 = attn_share(total, n_cta, cta + 1);
     AttnUnit u;
@@ -294,55 +299,53 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                 }
             }
             pg_proxy_fence();
-            if (!whole) __threadfence();
             pr_bar();
             if (lane == 0) pg_arrive(&sh.empty[st]);
             if (!whole) {
                 // ---- join the CTAs' states of this unit
                 const int ca = attn_owner(total, n_cta, attn_place(u, p, 0)), cb = attn_owner(total, n_cta, attn_place(u, p, u.steps - 1));
                 if (tid == 0) {
-                    sh.last = atomicAdd(&p.tickets[ca], 1u) == (unsigned)(cb - ca);
+                    sh.last = pg_ticket(&p.tickets[ca]) == (unsigned)(cb - ca);
                     if (sh.last) p.tickets[ca] = 0u;
-                    __threadfence();
                 }
                 pr_bar();
                 if (sh.last) {
-                    for (int r = warp; r < u.rows; r += PR_WARPS) {
-                        float M = -INFINITY, L = 0.f;
-                        for (int c = ca + lane; c <= cb; c += 32) {
-                            const int sl = 2 * c + (c == ca ? 1 : 0);
-                            M = fmaxf(M, __ldcg(&p.part_ml[(sl * PR_ROWS + r) * 2]));
-                        }
-#pragma unroll
-                        for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-                        const float base = M == -INFINITY ? 0.f : M;
-                        for (int c = ca + lane; c <= cb; c += 32) {
-                            const int sl = 2 * c + (c == ca ? 1 : 0);
-                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml) + sl * PR_ROWS + r);
-                            L = fmaf(exp2f(ml.x - base), ml.y, L);
-                        }
-#pragma unroll
-                        for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
-                        if (lane == 0) {
-                            sh.row_m[r] = base;
-                            sh.row_l[r] = L;
-                        }
-                    }
-                    pr_bar();
                     for (int i = tid; i < u.rows * C4; i += 32 * PR_WARPS) {
+                        // eight states at a time, their loads all in flight together
+                        constexpr int W = 8;
                         const int r = i / C4, c4 = i % C4;
-                        const float base = sh.row_m[r], inv = 1.f / sh.row_l[r];
+                        const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + r;
+                        const float4 *po = reinterpret_cast<const float4 *>(p.part_o) + r * C4 + c4;
+                        float M = -INFINITY, L = 0.f;
                         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                        for (int c = ca; c <= cb; c++) {
-                            const int sl = 2 * c + (c == ca ? 1 : 0);
-                            const float f = exp2f(__ldcg(&p.part_ml[(sl * PR_ROWS + r) * 2]) - base);
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.part_o) + ((long long)sl * PR_ROWS + r) * C4 + c4);
-                            a.x = fmaf(f, v.x, a.x);
-                            a.y = fmaf(f, v.y, a.y);
-                            a.z = fmaf(f, v.z, a.z);
-                            a.w = fmaf(f, v.w, a.w);
+                        for (int c = ca; c <= cb; c += W) {
+                            float2 s[W];
+                            float4 v[W];
+#pragma unroll
+                            for (int k = 0; k < W; k++) {
+                                const int sl = 2 * min(c + k, cb) + (min(c + k, cb) == ca ? 1 : 0);
+                                s[k] = __ldcg(ml + sl * PR_ROWS);
+                                v[k] = __ldcg(po + (long long)sl * (PR_ROWS * C4));
+                            }
+                            float mn = M;
+#pragma unroll
+                            for (int k = 0; k < W; k++) mn = fmaxf(mn, s[k].x);
+                            const float base = mn == -INFINITY ? 0.f : mn, f0 = exp2f(M - base);
+                            M = mn;
+                            L *= f0;
+                            a = make_float4(a.x * f0, a.y * f0, a.z * f0, a.w * f0);
+#pragma unroll
+                            for (int k = 0; k < W; k++) {
+                                if (c + k > cb) break;
+                                const float f = exp2f(s[k].x - base);
+                                L = fmaf(f, s[k].y, L);
+                                a.x = fmaf(f, v[k].x, a.x);
+                                a.y = fmaf(f, v[k].y, a.y);
+                                a.z = fmaf(f, v[k].z, a.z);
+                                a.w = fmaf(f, v[k].w, a.w);
+                            }
                         }
+                        const float inv = 1.f / L;
                         const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
                         const bool sees = p0 + t >= 0;
                         a = sees ? make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);

@@ -241,15 +241,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pg_saddr(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (tid == 32 * 9) {
+        pg_prefetch_map(&p.kmap);
+        pg_prefetch_map(&p.vmap);
+        pg_prefetch_map(&p.qmap);
+    }
+    pt_fence_before();
+    __syncthreads();
+    pt_fence_after();
     pdl_trigger();
     pdl_wait();
     const int rt = pt_tile_rows(p.group), ru = 2 * rt;
-    pt_fence_before();
-    const uint32_t total = attn_plan_build<PT_THREADS>(sh.plan, p, ru, PT_BK_SHIFT);  // ends with a barrier
-    pt_fence_after();
+    uint32_t longest;
+    const uint32_t total = attn_plan_build<PT_THREADS>(sh.plan, p, ru, PT_BK_SHIFT, longest);
     constexpr uint32_t tmem = 0;  // all 512 columns
     if (sh.tmem != tmem && tid == 0) *p.status = 2;
-    const int n_cta = attn_ctas(p, total), cta = blockIdx.x;
+    const int n_cta = attn_ctas(p, total, longest), cta = blockIdx.x;
 
     // 384 threads at 168 registers: the softmax warpgroups take 224 each, the third keeps 56
     if (warp >= 8) {
@@ -647,14 +654,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                             for (int j = 0; j < 32; j += 4) po[(c + j) / 4 * 128] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                         }
                 }
-                __threadfence();
                 __syncwarp();
                 if (lane == 0) pg_arrive(&sh.join);
                 pg_wait(&sh.join, nj++ & 1, &sh.fail);
                 if (tid == 0) {
-                    sh.last = atomicAdd(&p.tickets[w.ca], 1u) == (unsigned)(w.cb - w.ca);
+                    sh.last = pg_ticket(&p.tickets[w.ca]) == (unsigned)(w.cb - w.ca);
                     if (sh.last) p.tickets[w.ca] = 0u;
-                    __threadfence();
                 }
                 __syncwarp();
                 if (lane == 0) pg_arrive(&sh.join);
