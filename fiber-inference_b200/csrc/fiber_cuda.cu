@@ -28,6 +28,7 @@
 
 #include "attention.cuh"
 #include "fiber_cuda.h"
+#include "fiber_paged.h"
 #include "gemv.cuh"
 #include "gemv_tc.cuh"
 #include "launch.cuh"
@@ -435,6 +436,11 @@ struct gpu_context {
     int g_batch_n = 0;
     float *att_ws = nullptr;           // page-split attention states (batched layer pass)
     unsigned int *att_tickets = nullptr;
+    // ragged pass (prompt chunks and single tokens of several slots; fiber_paged.h)
+    int32_t *rg_meta = nullptr;        // q_start [max_batch + 1], kv_len [max_batch], slot [max_batch]
+    uint16_t *rg_q = nullptr, *rg_att = nullptr;  // fp16 [PF_CHUNK][heads * head_dim]: rotated queries, attention
+    void *rg_ws = nullptr;             // fiber_attn_paged's workspace
+    size_t rg_ws_bytes = 0;
     std::vector<void *> pf_pad;        // Q6_K matrices re-laid with 16-byte-aligned rows
     unsigned long long *smp_rng = nullptr;  // device sampler state (sampling decode loop)
     int32_t *smp_out = nullptr;
@@ -462,7 +468,7 @@ extern "C" void fiber_cuda_free(fiber_ctx_t *c) {
     if (c->ar_epoch) cudaFree(c->ar_epoch);
     if (c->comm) ncclCommDestroy(c->comm);
     for (void *q : c->pf_pad) cudaFree(q);
-    void *dev[] = {c->pf_x2, c->smp_rng, c->smp_out, c->att_ws, c->att_tickets, c->bt_pos, c->bt_arg, c->bt_rec, c->bt_step, c->bt_logits, c->pf_x, c->pf_qkv, c->pf_att, c->pf_hg, c->pf_hu, c->pf_bp, c->pf_tok, c->x2, c->d_shard, c->d_data, c->x, c->qkv, c->att, c->h, c->logits, c->rope, c->io, c->rec,
+    void *dev[] = {c->rg_meta, c->rg_q, c->rg_att, c->rg_ws, c->pf_x2, c->smp_rng, c->smp_out, c->att_ws, c->att_tickets, c->bt_pos, c->bt_arg, c->bt_rec, c->bt_step, c->bt_logits, c->pf_x, c->pf_qkv, c->pf_att, c->pf_hg, c->pf_hu, c->pf_bp, c->pf_tok, c->x2, c->d_shard, c->d_data, c->x, c->qkv, c->att, c->h, c->logits, c->rope, c->io, c->rec,
                    c->att_part, c->att_cnt, c->am_part, c->am_cnt, c->d_phases, c->d_bar,
                    c->d_fphases, c->fl_words, c->fl_sync, c->fl_att_words, c->fl_am,
                    c->pk_gf[0], c->pk_gf[1], c->pk_gf[2], c->pk_gf[3], c->pk_ss[0], c->pk_ss[1]};
@@ -1780,11 +1786,13 @@ static cudaError_t launch_g5_pack(const G5PackParams &a, cudaStream_t st) {
     return launch_pdl(g5_pack_kernel, grid, dim3(128), 0, st, a);
 }
 
-// Pack n rows of x (RMS-normalised with weights nw when given) into c->pf_bp.
-static cudaError_t pf_pack(gpu_context *c, const float *x, int cols, const float *nw, int n, cudaStream_t st) {
+// Pack n rows of x (RMS-normalised with weights nw when given), or of x16 (fp16), into c->pf_bp.
+static cudaError_t pf_pack(gpu_context *c, const float *x, int cols, const float *nw, int n, cudaStream_t st,
+                           const uint16_t *x16 = nullptr) {
     G5PackParams a;
     memset(&a, 0, sizeof(a));
     a.x = x;
+    a.x16 = x16;
     a.ldx = cols;
     a.ntok = n;
     a.cols = cols;
@@ -1821,8 +1829,11 @@ static cudaError_t pf_gemm(gpu_context *c, const CUtensorMap &map, const uint8_t
 // The layers over `n` tokens whose hidden states are in c->pf_x, each at its place
 // (position, KV slot): per layer RMSNorm + packing of the input, QKV GEMMs, RoPE + KV
 // append, causal attention, Wo GEMM (+residual), RMSNorm + packing, gate/up GEMMs,
-// SwiGLU, down GEMM (+residual).
-static cudaError_t enqueue_layers(gpu_context *c, const kv_cache_t *kv, int n, const TokenPlace &at, cudaStream_t st) {
+// SwiGLU, down GEMM (+residual). With `ragged` the tokens belong to its sequences (at is
+// not used): append and attention are fiber_kv_append and fiber_attn_paged, on fp16
+// queries.
+static cudaError_t enqueue_layers(gpu_context *c, const kv_cache_t *kv, int n, const TokenPlace &at, cudaStream_t st,
+                                  const fiber_ragged_t *ragged = nullptr) {
     const model_params_t &p = c->p;
     // this rank's share (the whole model when tp_world == 1): query / KV heads, FFN rows
     const int dim = p.dim, hd = p.head_dim, qd = c->nh_l * hd, kvd = c->nkv_l * hd, ffn = c->ffn_l;
@@ -1844,39 +1855,51 @@ static cudaError_t enqueue_layers(gpu_context *c, const kv_cache_t *kv, int n, c
         if ((e = pf_gemm(c, mp[0], pw[0], d.tq, qd, dim, c->pf_qkv, ldq, 0, false, n, st))) break;
         if ((e = pf_gemm(c, mp[1], pw[1], d.tk, kvd, dim, c->pf_qkv, ldq, qd, false, n, st))) break;
         if ((e = pf_gemm(c, mp[2], pw[2], d.tv, kvd, dim, c->pf_qkv, ldq, qd + kvd, false, n, st))) break;
-        RopeKvParams rk;
-        rk.qkv = c->pf_qkv;
-        rk.ldq = ldq;
-        rk.at = at;
-        rk.rope = c->rope;
-        rk.n_heads = c->nh_l;
-        rk.n_kv = c->nkv_l;
-        rk.hd = hd;
-        rk.k_pool = kv->k_pool;
-        rk.v_pool = kv->v_pool;
-        rk.page_table = kv->page_table;
-        rk.layer = l;
-        rk.n_layers = p.n_layers;
-        rope_kv_kernel<<<n, 256, 0, st>>>(rk);
-        if ((e = cudaGetLastError()) != cudaSuccess) break;
-        AttnPrefillParams ap;
-        ap.qkv = c->pf_qkv;
-        ap.ldq = ldq;
-        ap.out = c->pf_att;
-        ap.ldo = qd;
-        ap.at = at;
-        ap.k_pool = kv->k_pool;
-        ap.v_pool = kv->v_pool;
-        ap.page_table = kv->page_table;
-        ap.layer = l;
-        ap.n_layers = p.n_layers;
-        ap.n_kv = c->nkv_l;
-        ap.n_heads = c->nh_l;
-        ap.scale = 1.0f / sqrtf((float)hd);
-        ap.part = c->att_ws;
-        ap.tickets = c->att_tickets;
-        if ((e = launch_attn_prefill(c, ap, n, st))) break;
-        if ((e = pf_pack(c, c->pf_att, qd, nullptr, n, st))) break;
+        if (ragged) {
+            fiber_kv_view_t view;
+            const fiber_rope_t rope = {(const float *)c->rope, c->max_seq, hd, 0};
+            if (fiber_kv_view(kv, (int)l, &view) ||
+                fiber_kv_append(&view, ragged, FIBER_TYPE_F32, c->pf_qkv, ldq, c->pf_qkv + qd, ldq, c->pf_qkv + qd + kvd, ldq,
+                                c->nh_l, &rope, c->rg_q, qd, st) ||
+                fiber_attn_paged(&view, ragged, c->rg_q, qd, c->rg_att, qd, c->nh_l, 1.0f / sqrtf((float)hd), 0, c->rg_ws,
+                                 c->rg_ws_bytes, st))
+                return cudaErrorUnknown;  // fiber_last_error() has the reason
+            if ((e = pf_pack(c, nullptr, qd, nullptr, n, st, c->rg_att))) break;
+        } else {
+            RopeKvParams rk;
+            rk.qkv = c->pf_qkv;
+            rk.ldq = ldq;
+            rk.at = at;
+            rk.rope = c->rope;
+            rk.n_heads = c->nh_l;
+            rk.n_kv = c->nkv_l;
+            rk.hd = hd;
+            rk.k_pool = kv->k_pool;
+            rk.v_pool = kv->v_pool;
+            rk.page_table = kv->page_table;
+            rk.layer = l;
+            rk.n_layers = p.n_layers;
+            rope_kv_kernel<<<n, 256, 0, st>>>(rk);
+            if ((e = cudaGetLastError()) != cudaSuccess) break;
+            AttnPrefillParams ap;
+            ap.qkv = c->pf_qkv;
+            ap.ldq = ldq;
+            ap.out = c->pf_att;
+            ap.ldo = qd;
+            ap.at = at;
+            ap.k_pool = kv->k_pool;
+            ap.v_pool = kv->v_pool;
+            ap.page_table = kv->page_table;
+            ap.layer = l;
+            ap.n_layers = p.n_layers;
+            ap.n_kv = c->nkv_l;
+            ap.n_heads = c->nh_l;
+            ap.scale = 1.0f / sqrtf((float)hd);
+            ap.part = c->att_ws;
+            ap.tickets = c->att_tickets;
+            if ((e = launch_attn_prefill(c, ap, n, st))) break;
+            if ((e = pf_pack(c, c->pf_att, qd, nullptr, n, st))) break;
+        }
         // residual stream after Wo: pf_x (single GPU) or pf_x2 (sum over the ranks)
         float *xa = tp ? c->pf_x2 : c->pf_x;
         if (tp) {
@@ -2126,6 +2149,99 @@ static int forward_batch(gpu_context *c, kv_cache_t *kv, const int32_t *tokens, 
         CK(cudaMemcpyAsync(argmax_or_null, c->bt_arg, (size_t)batch * 4, cudaMemcpyDeviceToHost, c->stream));
     CK(cudaMemcpyAsync(c->h_io, c->io, sizeof(StepIO), cudaMemcpyDeviceToHost, c->stream));
     CK(cudaStreamSynchronize(c->stream));
+    return batch_status(c);
+}
+
+// ---- ragged pass: prompt chunks and single tokens of several slots ---------------------
+
+static int rg_alloc(gpu_context *c, const kv_cache_t *kv) {
+    int rc = pf_alloc(c);
+    if (rc || c->rg_ws) return rc;
+    fiber_kv_view_t view;
+    if ((rc = fiber_kv_view(kv, 0, &view))) return rc;
+    const fiber_ragged_t most = {c->max_batch, PF_CHUNK, PF_CHUNK, (const int32_t *)kv->page_table, kv->page_table, nullptr};
+    const fiber_ragged_t least = {c->max_batch, PF_CHUNK, 1, (const int32_t *)kv->page_table, kv->page_table, nullptr};
+    const size_t bytes = std::max(fiber_attn_paged_workspace(&view, &most, c->nh_l),
+                                  fiber_attn_paged_workspace(&view, &least, c->nh_l));
+    if (!bytes) return FIBER_EUNSUPPORTED;  // fiber_last_error() has the reason
+    const size_t row = (size_t)c->nh_l * c->p.head_dim * 2;
+    CK(cudaMalloc(&c->rg_meta, (3 * (size_t)c->max_batch + 1) * 4));
+    CK(cudaMalloc(&c->rg_q, PF_CHUNK * row));
+    CK(cudaMalloc(&c->rg_att, PF_CHUNK * row));
+    CK(cudaMalloc(&c->rg_ws, bytes));
+    CK(cudaMemset(c->rg_ws, 0, bytes));
+    c->rg_ws_bytes = bytes;
+    return FIBER_OK;
+}
+
+extern "C" int fiber_forward_ragged(fiber_ctx_t *c, kv_cache_t *kv, int n_seqs, const int32_t *slots,
+                                    const int32_t *start_pos, const int32_t *n_tokens, const int32_t *tokens,
+                                    float *logits_or_null, int32_t *argmax_or_null) {
+    if (!c || !kv || !slots || !start_pos || !n_tokens || !tokens)
+        return set_err(FIBER_EARG, "fiber_forward_ragged: null argument");
+    if (n_seqs < 1 || n_seqs > c->max_batch)
+        return set_err(FIBER_EARG, "fiber_forward_ragged: %d sequences outside [1, max_batch %d]", n_seqs, c->max_batch);
+    if (!batched_ok(c))
+        return set_err(FIBER_EUNSUPPORTED, "fiber_forward_ragged: the batched layer pass does not cover this model");
+    int rc = check_kv(c, kv);
+    if (rc) return rc;
+    const int lim = c->max_seq < kv->max_seq ? c->max_seq : kv->max_seq, B = c->max_batch;
+    std::vector<int32_t> meta(3 * (size_t)B + 1, 0);  // q_start, kv_len, slot
+    int n = 0, longest = 0;
+    for (int s = 0; s < n_seqs; s++) {
+        const int m = n_tokens[s];
+        if (slots[s] < 0 || slots[s] >= kv->max_batch)
+            return set_err(FIBER_EARG, "fiber_forward_ragged: no slot %d", slots[s]);
+        for (int o = 0; o < s; o++)
+            if (slots[o] == slots[s]) return set_err(FIBER_EARG, "fiber_forward_ragged: slot %d given twice", slots[s]);
+        if (m < 1 || m > PF_CHUNK - n)
+            return set_err(FIBER_EARG, "fiber_forward_ragged: sequence %d: %d tokens (1 .. %d of all sequences in one pass)", s,
+                           m, PF_CHUNK);
+        if (start_pos[s] < 0 || start_pos[s] > lim - m)
+            return set_err(FIBER_EARG, "fiber_forward_ragged: sequence %d: positions %d..%d outside [0, %d)", s, start_pos[s],
+                           start_pos[s] + m - 1, lim);
+        n += m;
+        longest = std::max(longest, m);
+        meta[s + 1] = n;
+        meta[B + 1 + s] = start_pos[s] + m;
+        meta[2 * B + 1 + s] = slots[s];
+    }
+    for (int i = 0; i < n; i++)
+        if (tokens[i] < 0 || tokens[i] >= (int)c->p.vocab_size)
+            return set_err(FIBER_EARG, "fiber_forward_ragged: token %d out of range", tokens[i]);
+    CK(cudaSetDevice(c->device));
+    if ((rc = rg_alloc(c, kv))) return rc;
+    const int dim = c->p.dim, V = c->p.vocab_size;
+    c->h_io->err = 0;
+    CK(cudaMemcpyAsync(c->io, c->h_io, sizeof(StepIO), cudaMemcpyHostToDevice, c->stream));
+    CK(cudaMemcpyAsync(c->pf_tok, tokens, (size_t)n * 4, cudaMemcpyHostToDevice, c->stream));
+    CK(cudaMemcpyAsync(c->rg_meta, meta.data(), meta.size() * 4, cudaMemcpyHostToDevice, c->stream));
+    const fiber_ragged_t batch = {n_seqs, n, longest, c->rg_meta, c->rg_meta + B + 1, c->rg_meta + 2 * B + 1};
+    const TokenPlace none = place_of(c, kv);
+    cudaError_t e = launch_embed_rows(c, c->pf_tok, c->pf_x, n, c->stream);
+    if (e == cudaSuccess) e = enqueue_layers(c, kv, n, none, c->stream, &batch);
+    if (e == cudaErrorUnknown)  // an operator refused (its message stands), or an exchange failed
+        return c->tp_world > 1 ? set_err(FIBER_ECUDA, "ragged pass: an exchange between the ranks or an operator failed") : FIBER_ECUDA;
+    if (e == cudaSuccess) {  // final RMSNorm + classifier on each sequence's last token
+        last_rows_kernel<<<n_seqs, 256, 0, c->stream>>>(c->pf_x, c->rg_meta, c->pf_att, dim);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) e = pf_pack(c, c->pf_att, dim, c->out_norm, n_seqs, c->stream);
+    if (e == cudaSuccess) e = pf_gemm(c, c->out_map, c->pf_out, c->t_out, V, dim, c->bt_logits, V, 0, false, n_seqs, c->stream);
+    if (e == cudaSuccess) {
+        argmax_rows_kernel<<<n_seqs, 256, 0, c->stream>>>(c->bt_logits, V, V, c->bt_arg);
+        e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) return set_err(FIBER_ECUDA, "ragged pass: %s", cudaGetErrorString(e));
+    if (logits_or_null)
+        CK(cudaMemcpyAsync(logits_or_null, c->bt_logits, (size_t)n_seqs * V * 4, cudaMemcpyDeviceToHost, c->stream));
+    if (argmax_or_null)
+        CK(cudaMemcpyAsync(argmax_or_null, c->bt_arg, (size_t)n_seqs * 4, cudaMemcpyDeviceToHost, c->stream));
+    CK(cudaMemcpyAsync(c->h_io, c->io, sizeof(StepIO), cudaMemcpyDeviceToHost, c->stream));
+    if ((rc = fiber_attn_paged_status(c->rg_ws, c->stream))) {
+        cudaMemset(c->rg_ws, 0, c->rg_ws_bytes);
+        return rc;
+    }
     return batch_status(c);
 }
 

@@ -172,6 +172,7 @@ FDEV void g5_cluster_sync() {
 
 struct G5PackParams {
     const float *x;        // [ntok][ldx]
+    const uint16_t *x16;   // the same as fp16 bits, in place of x (no normalisation then), or null
     int ldx, ntok, cols;
     const float *rrms;     // [ntok] or null: 1 / rms per token
     const float *nw;       // [cols] or null: no normalisation
@@ -368,9 +369,18 @@ __global__ void __launch_bounds__(128) g5_pack_kernel(const G5PackParams a) {
         const int i = tid + 128 * it, g = (col0 >> 3) + (i >> 3), nr = i & 7, tt = nr >> 1, t = t0 + tt;
         uint4 out = make_uint4(0u, 0u, 0u, 0u);
         if (t < a.ntok) {
-            const float4 *xp = reinterpret_cast<const float4 *>(a.x + (size_t)t * a.ldx + 8 * g);
-            const float4 x0 = xp[0], x1 = xp[1];
-            float v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+            float v[8];
+            if (a.x16) {
+                const uint4 xh = *reinterpret_cast<const uint4 *>(a.x16 + (size_t)t * a.ldx + 8 * g);
+                const uint32_t w[4] = {xh.x, xh.y, xh.z, xh.w};
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = h2f(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]);
+            } else {
+                const float4 *xp = reinterpret_cast<const float4 *>(a.x + (size_t)t * a.ldx + 8 * g);
+                const float4 x0 = xp[0], x1 = xp[1];
+                v[0] = x0.x, v[1] = x0.y, v[2] = x0.z, v[3] = x0.w;
+                v[4] = x1.x, v[5] = x1.y, v[6] = x1.z, v[7] = x1.w;
+            }
             if (a.nw) {
                 const float4 n0 = reinterpret_cast<const float4 *>(a.nw + 8 * g)[0];
                 const float4 n1 = reinterpret_cast<const float4 *>(a.nw + 8 * g)[1];

@@ -10,6 +10,7 @@
 //   swiglu_rows_kernel  h = silu(gate) * up
 //   argmax_rows_kernel  greedy token of each logits row (lowest index on ties)
 //   batch_advance_kernel  device-resident greedy loop: argmax -> next token, pos + 1
+//   last_rows_kernel    hidden state of each sequence's last token (ragged pass)
 #pragma once
 #include "attention.cuh"
 
@@ -343,6 +344,12 @@ __global__ void swiglu_rows_kernel(float *hg, const float *__restrict__ hu, size
         const float g = hg[i];
         hg[i] = __fmul_rn(__fdiv_rn(g, __fadd_rn(1.0f, expf(-g))), hu[i]);
     }
+}
+
+// One CTA per sequence: the row of its last token, out[s] = X[q_start[s + 1] - 1].
+__global__ void last_rows_kernel(const float *__restrict__ X, const int32_t *__restrict__ q_start, float *out, int dim) {
+    const size_t from = (size_t)(q_start[blockIdx.x + 1] - 1) * dim, to = (size_t)blockIdx.x * dim;
+    for (int i = threadIdx.x; i < dim; i += blockDim.x) out[to + i] = X[from + i];
 }
 
 // One CTA (256 threads) per row: index of the maximum, the lowest index winning ties

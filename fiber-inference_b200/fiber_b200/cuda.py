@@ -31,7 +31,8 @@ EXPORTED = [
     "gpu_get_logits", "gpu_forward_classifier", "gpu_get_device", "kv_cache_init", "kv_cache_init_paged",
     "kv_cache_free", "kv_cache_write", "kv_cache_read", "fiber_gemv_argmax_noalloc", "fiber_prefill_slot",
     "fiber_decode_greedy_batch", "fiber_sample", "fiber_decode_sample", "fiber_tp_collective", "fiber_set_max_batch",
-    "fiber_step_ring_bytes",
+    "fiber_step_ring_bytes", "fiber_forward_ragged", "fiber_kv_view", "fiber_kv_append", "fiber_attn_paged",
+    "fiber_attn_paged_workspace", "fiber_attn_paged_status",
 ]
 
 
@@ -73,6 +74,7 @@ def cuda_lib() -> C.CDLL:
         L.fiber_prefill_slot.argtypes = [C.c_void_p, C.c_void_p, C.c_int, I32P, C.c_int, C.c_int, C.c_void_p]
         L.fiber_decode_greedy_batch.argtypes = [C.c_void_p, C.c_void_p, I32P, I32P, C.c_int, C.c_int, C.c_void_p,
                                                 C.c_void_p]
+        L.fiber_forward_ragged.argtypes = [C.c_void_p, C.c_void_p, C.c_int, I32P, I32P, I32P, I32P, C.c_void_p, C.c_void_p]
         L.fiber_sample.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, C.c_float, C.c_void_p,
                                    C.c_void_p, C.c_void_p]
         L.fiber_decode_sample.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_int, C.c_int, C.c_float, C.c_int,
@@ -294,6 +296,19 @@ class Context:
         _check(cuda_lib().fiber_forward_token(self.h, kv.addr, t, p, len(t),
                                               lg.ctypes.data if lg is not None else None, am.ctypes.data),
                "fiber_forward_token")
+        return am, lg
+
+    def forward_ragged(self, kv: KVCache, slots, start_pos, chunks, want_logits: bool = True):
+        """One pass over a chunk of tokens (one or more) per sequence, sequence i on KV slot
+        slots[i] from position start_pos[i]: (greedy token after each chunk, logits or None)."""
+        n = np.array([len(c) for c in chunks], np.int32)
+        t = np.ascontiguousarray(np.concatenate([np.asarray(c, np.int32).ravel() for c in chunks]), np.int32)
+        lg = np.empty((len(n), self.p.vocab_size), np.float32) if want_logits else None
+        am = np.zeros(len(n), np.int32)
+        _check(cuda_lib().fiber_forward_ragged(self.h, kv.addr, len(n), np.ascontiguousarray(slots, np.int32),
+                                               np.ascontiguousarray(start_pos, np.int32), n, t,
+                                               lg.ctypes.data if lg is not None else None, am.ctypes.data),
+               "fiber_forward_ragged")
         return am, lg
 
     def decode_greedy_batch(self, kv: KVCache, first_tokens, start_pos, n_steps: int):

@@ -89,6 +89,19 @@ int fiber_decode_greedy_batch(fiber_ctx_t *ctx, kv_cache_t *kv, const int32_t *f
                               const int32_t *start_pos, int batch, int n_steps, int32_t *h_tokens_out,
                               float *ms_out);
 
+/* One pass over tokens of several sequences at once, prompt chunks and single decode
+ * tokens mixed: sequence i (of n_seqs, 1 .. max_batch) brings n_tokens[i] >= 1 tokens
+ * (one after the other in `tokens`) at positions start_pos[i] .. of KV slot slots[i] (each
+ * slot once); all sequences together at most FIBER_PREFILL_CHUNK tokens. Appends their keys
+ * and values and returns, if non-NULL, the fp32 logits [n_seqs][vocab] and the greedy token
+ * of each sequence's last token. Host arrays; blocks until done. Attention runs on the
+ * tensor cores over the paged cache (fiber_paged.h): queries, probabilities and its output
+ * are rounded to fp16 there, the cache holds the bits of the other paths. No counterpart in
+ * the reference (one sequence, token by token). */
+int fiber_forward_ragged(fiber_ctx_t *ctx, kv_cache_t *kv, int n_seqs, const int32_t *slots,
+                         const int32_t *start_pos, const int32_t *n_tokens, const int32_t *tokens,
+                         float *logits_or_null, int32_t *argmax_or_null);
+
 /* Sampling on the device with the reference sampler's procedure (src/sampler.c:48-112):
  * temperature <= 0 (or < 1e-6) is the greedy argmax; otherwise logits * (1/T), the
  * top_k (top_k <= 0: all) largest sorted descending (equal values in index order; with
