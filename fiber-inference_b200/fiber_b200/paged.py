@@ -83,14 +83,16 @@ def kv_view(cache, layer: int) -> PagedKV:
     return view
 
 
-def kv_append(kv: PagedKV, batch: RaggedBatch, in_type: int, q: int | None, k: int, v: int, *, ld: int | None = None,
+def kv_append(kv: PagedKV, batch: RaggedBatch, in_type: int, q: int | None, k: int, v: int, *, ld: int = 0,
               ldq: int | None = None, ldk: int | None = None, ldv: int | None = None, n_heads: int = 0,
               q_out: int | None = None, ld_out: int = 0, rope: Rope | None = None, stream=None):
     """fiber_kv_append: q rotated into q_out, k rotated and v into the cache. `ld` is the row
     stride of q, k and v alike (one fused buffer); ldq / ldk / ldv set them apart."""
-    _check(_paged_lib().fiber_kv_append(kv, batch, in_type, q, (ld if ldq is None else ldq) or 0, k,
-                                        (ld if ldk is None else ldk) or 0, v, (ld if ldv is None else ldv) or 0, n_heads,
-                                        rope, q_out, ld_out, _stream_ptr(stream)), "fiber_kv_append")
+    rc = (_lib or _paged_lib()).fiber_kv_append(
+        kv, batch, in_type, q, ld if ldq is None else ldq, k, ld if ldk is None else ldk, v, ld if ldv is None else ldv,
+        n_heads, rope, q_out, ld_out, stream if type(stream) is int else _stream_ptr(stream))
+    if rc:
+        _check(rc, "fiber_kv_append")
 
 
 def attn_paged_workspace(kv: PagedKV, batch: RaggedBatch, n_heads: int) -> int:
@@ -104,8 +106,10 @@ def attn_paged_workspace(kv: PagedKV, batch: RaggedBatch, n_heads: int) -> int:
 def attn_paged(kv: PagedKV, batch: RaggedBatch, q: int, out: int, *, n_heads: int, ldq: int, ldo: int, scale: float,
                ws: int, ws_bytes: int, window: int = 0, stream=None):
     """fiber_attn_paged: causal attention of the batch's tokens over the cache."""
-    _check(_paged_lib().fiber_attn_paged(kv, batch, q, ldq, out, ldo, n_heads, scale, window, ws, ws_bytes,
-                                         _stream_ptr(stream)), "fiber_attn_paged")
+    rc = (_lib or _paged_lib()).fiber_attn_paged(kv, batch, q, ldq, out, ldo, n_heads, scale, window, ws, ws_bytes,
+                                                 stream if type(stream) is int else _stream_ptr(stream))
+    if rc:
+        _check(rc, "fiber_attn_paged")
 
 
 def attn_paged_status(ws: int, stream=None):
