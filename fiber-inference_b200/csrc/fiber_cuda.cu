@@ -2186,7 +2186,7 @@ extern "C" int fiber_forward_ragged(fiber_ctx_t *c, kv_cache_t *kv, int n_seqs, 
     int rc = check_kv(c, kv);
     if (rc) return rc;
     const int lim = c->max_seq < kv->max_seq ? c->max_seq : kv->max_seq, B = c->max_batch;
-    std::vector<int32_t> meta(3 * (size_t)B + 1, 0);  // q_start, kv_len, slot
+    int32_t meta[3 * FIBER_MAX_BATCH + 1] = {};  // q_start [B + 1], kv_len [B], slot [B]
     int n = 0, longest = 0;
     for (int s = 0; s < n_seqs; s++) {
         const int m = n_tokens[s];
@@ -2215,7 +2215,7 @@ extern "C" int fiber_forward_ragged(fiber_ctx_t *c, kv_cache_t *kv, int n_seqs, 
     c->h_io->err = 0;
     CK(cudaMemcpyAsync(c->io, c->h_io, sizeof(StepIO), cudaMemcpyHostToDevice, c->stream));
     CK(cudaMemcpyAsync(c->pf_tok, tokens, (size_t)n * 4, cudaMemcpyHostToDevice, c->stream));
-    CK(cudaMemcpyAsync(c->rg_meta, meta.data(), meta.size() * 4, cudaMemcpyHostToDevice, c->stream));
+    CK(cudaMemcpyAsync(c->rg_meta, meta, (3 * (size_t)B + 1) * 4, cudaMemcpyHostToDevice, c->stream));
     const fiber_ragged_t batch = {n_seqs, n, longest, c->rg_meta, c->rg_meta + B + 1, c->rg_meta + 2 * B + 1};
     const TokenPlace none = place_of(c, kv);
     cudaError_t e = launch_embed_rows(c, c->pf_tok, c->pf_x, n, c->stream);

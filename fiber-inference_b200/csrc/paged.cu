@@ -324,7 +324,7 @@ extern "C" int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t 
     p.group = n_heads / kv->n_kv_heads;
     p.by_group = make_div((uint32_t)p.group);
     p.by_ru = make_div(shape.tile ? 2u * pt_tile_rows(p.group) : (unsigned)PR_ROWS);
-    p.window = window;
+    p.window = window >= kv->max_pages * kv->page_size ? 0 : window;  // wider than a slot: no window
     p.cost = shape.tile ? PT_COST : PR_COST;
     p.scale = scale;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);

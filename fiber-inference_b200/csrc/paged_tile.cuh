@@ -7,16 +7,22 @@
 //               maximum and sum, probabilities back to tensor memory in 16 bits
 //   warps 4-7   the same for tile B
 //   warps 8, 11 issue the MMAs of tile A and of tile B: S = Q K^T (operands in shared
-//               memory), then O += P V with P read from tensor memory (one warp for both
-//               left the tensor core idle for about 190 cycles at every hand-over)
+//               memory), then O += P V with P read from tensor memory (with one warp for
+//               both a step took 4,590 cycles: every wait of one tile also held up the other)
 //   warp 9      producer: Q, K and V tiles by TMA (K / V boxes go page by page)
 //   warp 10     scheduler: works out the CTA's units ahead of the others
 // Tensor memory: S_A, S_B (128 columns each), O_A, O_B (head_dim columns each). A key tile
 // is worked through in two halves of 64 keys, each with its own 64 columns of S, whose
 // front half its probabilities overwrite: while the softmax of one half runs, the tensor
 // core multiplies the other half's probabilities with V and computes its next scores, so
-// a softmax warp finds its next scores ready. (With one 128-key S per tile a step was the
-// sum of softmax, two products and four hand-overs: 4,200 cycles instead of 2,900.)
+// a softmax warp finds its next scores ready.
+//
+// Bound by the softmax warps, then by power. A step of both tiles (128 keys, head_dim 128)
+// takes 3,760 cycles; its products alone are 2,560 (S of 64 keys is bound by reading Q and K
+// from shared memory: 48 cycles per MMA where the arithmetic is 32), 2,920 with the hand-overs.
+// One S of 128 keys per step needs 2,048 but puts products and softmax in a row: 3,880. 2,048
+// tokens after 14,005 positions take 435 us from a cool start (1,160 TFLOP/s) and 507 at
+// 1,000 W, where the clock falls to 1.5 GHz.
 //
 // The output accumulators are rescaled only when a row's maximum has grown by more than
 // 2^8 since the last time (the probabilities, at most 2^8, keep their 11 or 8 bits).
@@ -201,7 +207,8 @@ FDEV void pt_tie16(float *v) {
 FDEV uint32_t pt_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
 
 // Pairs of every 4 whose exponentials run on the FMA pipe instead of the special-function
-// unit, which alone would need 2 x 1,024 cycles per step beside 2,048 of the tensor core.
+// unit, which alone would need 2 x 1,024 cycles per step (2,048 tokens after 14,005
+// positions: none 465 us, one in four 435, two 451).
 constexpr int PT_POLY = 1;
 
 template <int HD, bool BF>

@@ -166,6 +166,23 @@ def test_attn_chunks(dim, heads, kv_heads, dtype):
     s.check()
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(33, 1), (64, 1), (128, 1), (127, 1), (96, 2)])
+def test_attn_wide_groups(heads, kv_heads):
+    """Up to 128 query heads per KV head: tiles of one to three tokens."""
+    s = Setup([(1, 70), (5, 40), (3, 2), (4, 130)], heads, kv_heads, 64, "f16", 32, seed=heads)
+    s.attend()
+    s.check()
+
+
+@pytest.mark.parametrize("nq", [1, 30])
+def test_attn_window_beyond_the_cache(nq):
+    """The widest window there is, with rows that see nothing: as without a window."""
+    s = Setup([(nq, 20), (nq, 100)], 2, 1, 64, window=2 ** 31 - 1, seed=nq)
+    s.attend()
+    s.window = 0
+    s.check()
+
+
 @pytest.mark.parametrize("layout", ["heads", "positions"])
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("lens", [SINGLES, CHUNKS], ids=["singles", "chunks"])
