@@ -25,7 +25,8 @@
 // 1,000 W, where the clock falls to 1.5 GHz.
 //
 // The output accumulators are rescaled only when a row's maximum has grown by more than
-// 2^8 since the last time (the probabilities, at most 2^8, keep their 11 or 8 bits).
+// 2^15 (fp16) or 2^40 (bf16) since the last time: a rescale waits for the product before
+// it and costs its 32 rows about 3,000 cycles.
 #pragma once
 #include "paged.cuh"
 
@@ -34,7 +35,11 @@ namespace fiber {
 constexpr int PT_ROWS = 128;                          // rows of a tile
 constexpr int PT_BK_SHIFT = 7, PT_BK = 1 << PT_BK_SHIFT;  // keys of a tile
 constexpr int PT_THREADS = 384;
-constexpr float PT_GROWTH = 8.f;  // powers of two a row's maximum may grow before O is rescaled
+// Powers of two a row's maximum may grow before O is rescaled. A larger probability is no less
+// exact, so only the range of the 16-bit type and of the fp32 sums limits it: 2^15 for fp16
+// (below 65,504); 2^40 for bf16 leaves 2^87 to the sums.
+template <bool BF>
+HDCE float pt_growth() { return BF ? 40.f : 15.f; }
 
 // Tokens and rows of a tile: whole tokens (all heads of the group).
 HDCE int pt_tile_rows(int group) { return PT_ROWS / group * group; }
@@ -552,7 +557,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 await(j);
                 fetch(j, v);
                 const float mt = arrived(j, v);
-                const bool grow = mt > m + PT_GROWTH || (m == -INFINITY && mt > m);
+                const bool grow = mt > m + pt_growth<BF>() || (m == -INFINITY && mt > m);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float mn = grow ? mt : m;
                     const float f = grow ? pt_exp2(m - mn) : 1.f;
