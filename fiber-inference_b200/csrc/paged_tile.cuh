@@ -178,13 +178,19 @@ FDEV uint64_t pt_add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+FDEV uint64_t pt_mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (added and
 // subtracted 1.5 * 2^23), 2^f by a minimax polynomial of degree 4 on [-1/2, 1/2] (Remez
-// exchange on the relative error, 2.7e-6 in fp32), n added to the exponent. x is clamped
-// to -126: what lies below is nothing beside the row's largest weight of at least 1.
+// exchange on the relative error, 2.7e-6 in fp32), times 2^n, whose bits are n + 127 in the
+// exponent. x is clamped to -127, whose 2^n is all zero bits: a masked key's weight has to
+// be exactly 0 (bf16 holds 2^-126, and values up to 2^127 would meet it).
 FDEV float2 pt_exp2_poly(float x0, float x1) {
     const uint64_t magic = pt_two(12582912.f, 12582912.f), minus = pt_two(-12582912.f, -12582912.f);
-    const uint64_t x = pt_two(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+    const uint64_t x = pt_two(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
     const uint64_t t = pt_add2(x, magic);
     const uint64_t n = pt_add2(t, minus);
     const uint64_t f = pt_fma2(n, pt_two(-1.f, -1.f), x);
@@ -192,9 +198,9 @@ FDEV float2 pt_exp2_poly(float x0, float x1) {
     y = pt_fma2(y, f, pt_two(0.240247443318367f, 0.240247443318367f));
     y = pt_fma2(y, f, pt_two(0.6931217908859253f, 0.6931217908859253f));
     y = pt_fma2(y, f, pt_two(0.9999992847442627f, 0.9999992847442627f));
-    const float2 v = pt_both(y), e = pt_both(t);
-    return make_float2(__uint_as_float(__float_as_uint(v.x) + (__float_as_uint(e.x) << 23)),
-                       __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(e.y) << 23)));
+    const float2 e = pt_both(t);
+    return pt_both(pt_mul2(y, pt_two(__uint_as_float((__float_as_uint(e.x) << 23) + 0x3f800000u),
+                                     __uint_as_float((__float_as_uint(e.y) << 23) + 0x3f800000u))));
 }
 // Completion of tensor-memory loads, tied to the registers they fill
 FDEV void pt_wait_ld(float *v) {

@@ -251,6 +251,26 @@ def test_attn_positions_behind_the_mask_do_not_matter(dim, heads, kv_heads, bad)
     assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
 
 
+@pytest.mark.parametrize("at", range(8))
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attn_largest_values_behind_the_mask_do_not_matter(dim, at):
+    """A weight behind the mask is exactly zero: values near bf16's largest there add nothing."""
+    torch = torch_()
+    lens, window = [(150, 200), (1, 90)], 30
+    s = Setup(lens, 8, 2, dim, "bf16", 16, window=window, seed=21)
+    j = 104 + at  # the first rows are before it, the last have it behind their window
+    page = int(s.table[s.order[0], j // 16])
+    s.v[page, :, j % 16] = 3e38
+    s.dv.copy_(s.v)
+    s.attend()
+    fb.attn_paged_status(s.ws.data_ptr())
+    want, tol = s.reference()
+    got = s.out.cpu().double()[:s.n, :8 * dim].reshape(s.n, 8, dim)
+    clean = torch.tensor([not i - window + 1 <= j <= i for i in range(50, 200)] + [True])
+    assert clean.sum() == 151 - window
+    assert ((got - want).abs() <= tol)[clean].all()
+
+
 @pytest.mark.parametrize("bad", [-1, 1 << 30])
 def test_attn_table_entries_outside_the_pool_read_as_zeros(bad):
     torch = torch_()
