@@ -183,14 +183,20 @@ FDEV uint64_t pt_mul2(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+FDEV float pt_max(float a, float b) {  // NaN if either is (fmaxf returns the other)
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (added and
 // subtracted 1.5 * 2^23), 2^f by a minimax polynomial of degree 4 on [-1/2, 1/2] (Remez
 // exchange on the relative error, 2.7e-6 in fp32), times 2^n, whose bits are n + 127 in the
 // exponent. x is clamped to -127, whose 2^n is all zero bits: a masked key's weight has to
 // be exactly 0 (bf16 holds 2^-126, and values up to 2^127 would meet it).
+// A score that is NaN stays NaN, so that its row is seen to need the exact pass.
 FDEV float2 pt_exp2_poly(float x0, float x1) {
     const uint64_t magic = pt_two(12582912.f, 12582912.f), minus = pt_two(-12582912.f, -12582912.f);
-    const uint64_t x = pt_two(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
+    const uint64_t x = pt_two(pt_max(x0, -127.f), pt_max(x1, -127.f));
     const uint64_t t = pt_add2(x, magic);
     const uint64_t n = pt_add2(t, minus);
     const uint64_t f = pt_fma2(n, pt_two(-1.f, -1.f), x);

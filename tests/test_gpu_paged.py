@@ -271,6 +271,29 @@ def test_attn_largest_values_behind_the_mask_do_not_matter(dim, at):
     assert ((got - want).abs() <= tol)[clean].all()
 
 
+@pytest.mark.parametrize("at", range(8))
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attn_keys_that_are_not_finite_are_seen(bad, dtype, at):
+    """One element of one key is not finite and every value is: the rows that see the key, and no
+    others, get what the formula gives."""
+    torch = torch_()
+    lens = [(60, 130), (1, 90)]
+    s = Setup(lens, 8, 2, 64, dtype, 16, seed=22)
+    for q, j in ((0, 96 + at), (1, 40 + at)):
+        s.k[int(s.table[s.order[q], j // 16]), :, j % 16, 5] = bad
+    s.dk.copy_(s.k)
+    s.attend()
+    fb.attn_paged_status(s.ws.data_ptr())
+    want, tol = s.reference()
+    got = s.out.cpu().double()[:s.n, :8 * 64].reshape(s.n, 8, 64)
+    nan = torch.isnan(want)
+    assert nan.any() and not nan.all()
+    assert torch.equal(torch.isnan(got), nan)
+    clean = torch.tensor([i < 96 + at for i in range(70, 130)] + [False])
+    assert ((got - want).abs() <= tol)[clean].all()
+
+
 @pytest.mark.parametrize("bad", [-1, 1 << 30])
 def test_attn_table_entries_outside_the_pool_read_as_zeros(bad):
     torch = torch_()
