@@ -548,8 +548,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
             auto hand_over = [&](int j) {
                 const int h = j & 1, tile0 = (w.kt0 + (j >> 1)) << PT_BK_SHIFT;
                 npv++;
-                if ((h == 0 || j == ab) && (tile0 < w.lo || tile0 + PT_BK > w.hi) && (t == 0 || j < w.ab[0] || j >= w.ae[0])) {
-                    // values no row of the unit sees may hold anything: weight 0 must meet 0 there
+                if ((h == 0 || j == ab) && (tile0 < w.lo || tile0 + PT_BK > w.hi)) {
+                    // values no row of the unit sees may hold anything: weight 0 must meet 0 there.
+                    // Each tile clears them before its own product: the tiles' products do not
+                    // wait for one another (zeros over the other tile's zeros change nothing).
                     const uint32_t vi = it + 2 * ((j >> 1) - w.b) + 1;
                     pg_wait(&sh.kvfull[vi % NST], vi / NST & 1, &sh.fail);
                     if (tile0 + row < w.lo || tile0 + row >= w.hi)

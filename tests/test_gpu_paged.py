@@ -294,6 +294,22 @@ def test_attn_keys_that_are_not_finite_are_seen(bad, dtype, at):
     assert ((got - want).abs() <= tol)[clean].all()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("window", [0, 25])
+def test_attn_same_bits_again(window, dtype):
+    """Two tiles of queries share each unit's K and V, whose first and last rows neither sees."""
+    torch = torch_()
+    lens = [(700, 1500), (333, 333), (90, 2000), (1, 3000)] * 3
+    s = Setup(lens, 64, 4, 64, dtype, 32, window=window, seed=23, fill=float("nan"))
+    s.attend()
+    first = s.out.clone()
+    assert torch.isfinite(first).all()
+    for _ in range(60):
+        s.attend()
+        assert torch.equal(s.out, first)
+    fb.attn_paged_status(s.ws.data_ptr())
+
+
 @pytest.mark.parametrize("bad", [-1, 1 << 30])
 def test_attn_table_entries_outside_the_pool_read_as_zeros(bad):
     torch = torch_()
