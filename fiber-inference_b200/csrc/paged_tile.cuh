@@ -21,7 +21,7 @@
 // takes 3,760 cycles; its products alone are 2,560 (S of 64 keys is bound by reading Q and K
 // from shared memory: 48 cycles per MMA where the arithmetic is 32), 2,920 with the hand-overs.
 // One S of 128 keys per step needs 2,048 but puts products and softmax in a row: 3,880. 2,048
-// tokens after 14,005 positions take 435 us from a cool start (1,160 TFLOP/s) and 507 at
+// tokens after 14,005 positions take 439 us from a cool start (1,150 TFLOP/s) and 509 at
 // 1,000 W, where the clock falls to 1.5 GHz.
 //
 // The output accumulators are rescaled only when a row's maximum has grown by more than
@@ -225,7 +225,7 @@ FDEV uint32_t pt_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) 
 
 // Pairs of every 4 whose exponentials run on the FMA pipe instead of the special-function
 // unit, which alone would need 2 x 1,024 cycles per step (2,048 tokens after 14,005
-// positions: none 465 us, one in four 435, two 451).
+// positions: none 470 us, one in four 439, two 454).
 constexpr int PT_POLY = 1;
 
 template <int HD, bool BF>
