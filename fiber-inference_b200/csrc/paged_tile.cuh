@@ -667,7 +667,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 float4 *po = reinterpret_cast<float4 *>(p.part_o) + (long long)ps * (HD / 4) * 128 + row;
                 float *pm = p.part_ml + ps * 256 + row;
                 if (!idle) {
-                    pm[0] = did ? m : -INFINITY;
+                    // scores all NaN leave no maximum but a sum: the join must not pass it over
+                    pm[0] = !did ? -INFINITY : l != 0.f ? fmaxf(m, -3.4e38f) : m;
                     pm[128] = l;
                     if (did)
 #pragma unroll

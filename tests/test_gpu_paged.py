@@ -294,6 +294,20 @@ def test_attn_keys_that_are_not_finite_are_seen(bad, dtype, at):
     assert ((got - want).abs() <= tol)[clean].all()
 
 
+@pytest.mark.parametrize("lens", [(1, 3000), (40, 3000)], ids=["single", "chunk"])
+@pytest.mark.parametrize("lo,hi", [(0, 128), (512, 1024), (0, 2950), (0, 3000)])
+def test_attn_parts_whose_keys_are_all_nan_are_joined(lo, hi, lens):
+    """Every row sees a NaN, also where a part of a divided unit holds nothing else."""
+    torch = torch_()
+    s = Setup([lens], 8, 1, 64, "f16", 16, seed=24)
+    for j in range(lo, hi):
+        s.k[int(s.table[s.order[0], j // 16]), :, j % 16] = float("nan")
+    s.dk.copy_(s.k)
+    s.attend()
+    fb.attn_paged_status(s.ws.data_ptr())
+    assert torch.isnan(s.out[:s.n, :8 * 64]).all()
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("window", [0, 25])
 def test_attn_same_bits_again(window, dtype):
