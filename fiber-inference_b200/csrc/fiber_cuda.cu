@@ -1761,16 +1761,16 @@ static bool g5_make_map(CUtensorMap *map, const uint8_t *w, int type, int rows, 
 
 // The weights as the GEMM reads them: w itself, or for Q6_K rows that are not a multiple
 // of 16 bytes long a copy with padded rows (kept in c->pf_pad, or handed to the caller
-// to free when c is null).
+// to free when c is null), laid out on the stream whose kernels read them.
 static cudaError_t g5_weights(gpu_context *c, const uint8_t *w, int type, int rows, int cols, const uint8_t **out,
-                              void **owned = nullptr) {
+                              cudaStream_t st, void **owned = nullptr) {
     const size_t rb = (size_t)cols / 256 * block_bytes(type), prb = g5_row_bytes(type, cols);
     *out = w;
     if (prb == rb) return cudaSuccess;
     void *d = nullptr;
     cudaError_t e = cudaMalloc(&d, prb * rows);
     if (e != cudaSuccess) return e;
-    e = cudaMemcpy2D(d, prb, w, rb, rb, rows, cudaMemcpyDeviceToDevice);
+    e = cudaMemcpy2DAsync(d, prb, w, rb, rb, rows, cudaMemcpyDeviceToDevice, st);
     if (e != cudaSuccess) {
         cudaFree(d);
         return e;
@@ -1972,7 +1972,8 @@ static cudaError_t enqueue_batch_step(gpu_context *c, const kv_cache_t *kv, int 
     return e;
 }
 
-// Buffers and tensor maps of the batched layer pass, made on first use.
+// Buffers and tensor maps of the batched layer pass, made on first use. What fills them is
+// enqueued on the context's stream, which does not wait for the legacy stream.
 static int pf_alloc(gpu_context *c) {
     if (c->pf_cap) return FIBER_OK;
     const model_params_t &p = c->p;
@@ -1994,7 +1995,7 @@ static int pf_alloc(gpu_context *c) {
     CK(cudaMalloc(&c->bt_logits, B * p.vocab_size * 4));
     CK(cudaMalloc(&c->att_ws, (size_t)ATT_PART_ENTRIES * c->G * (p.head_dim + 2) * 4));
     CK(cudaMalloc(&c->att_tickets, ATT_PART_ENTRIES * sizeof(unsigned int)));
-    CK(cudaMemset(c->att_tickets, 0, ATT_PART_ENTRIES * sizeof(unsigned int)));
+    CK(cudaMemsetAsync(c->att_tickets, 0, ATT_PART_ENTRIES * sizeof(unsigned int), c->stream));
     c->pf_maps.assign(7 * p.n_layers, CUtensorMap{});
     c->pf_w.assign(7 * p.n_layers, nullptr);
     // this rank's share: rows of Wq / Wk / Wv / W1 / W3, input columns of Wo / W2
@@ -2006,12 +2007,12 @@ static int pf_alloc(gpu_context *c) {
         const int rows[7] = {qd, kvd, kvd, dim, ffn, dim, ffn}, cols[7] = {dim, dim, dim, qd, dim, ffn, dim};
         for (int k = 0; k < 7; k++) {
             const uint8_t **pw = &c->pf_w[7 * l + k];
-            CK(g5_weights(c, ws[k], ts[k], rows[k], cols[k], pw));
+            CK(g5_weights(c, ws[k], ts[k], rows[k], cols[k], pw, c->stream));
             if (!g5_make_map(&c->pf_maps[7 * l + k], *pw, ts[k], rows[k], cols[k]))
                 return set_err(FIBER_ECUDA, "batched layer pass: cannot build the weight tensor maps");
         }
     }
-    CK(g5_weights(c, c->out, c->t_out, (int)p.vocab_size, dim, &c->pf_out));
+    CK(g5_weights(c, c->out, c->t_out, (int)p.vocab_size, dim, &c->pf_out, c->stream));
     if (!g5_make_map(&c->out_map, c->pf_out, c->t_out, (int)p.vocab_size, dim))
         return set_err(FIBER_ECUDA, "batched layer pass: cannot build the classifier tensor map");
     c->pf_cap = PF_CHUNK;
@@ -2169,7 +2170,7 @@ static int rg_alloc(gpu_context *c, const kv_cache_t *kv) {
     CK(cudaMalloc(&c->rg_q, PF_CHUNK * row));
     CK(cudaMalloc(&c->rg_att, PF_CHUNK * row));
     CK(cudaMalloc(&c->rg_ws, bytes));
-    CK(cudaMemset(c->rg_ws, 0, bytes));
+    CK(cudaMemsetAsync(c->rg_ws, 0, bytes, c->stream));
     c->rg_ws_bytes = bytes;
     return FIBER_OK;
 }
@@ -2239,7 +2240,7 @@ extern "C" int fiber_forward_ragged(fiber_ctx_t *c, kv_cache_t *kv, int n_seqs, 
         CK(cudaMemcpyAsync(argmax_or_null, c->bt_arg, (size_t)n_seqs * 4, cudaMemcpyDeviceToHost, c->stream));
     CK(cudaMemcpyAsync(c->h_io, c->io, sizeof(StepIO), cudaMemcpyDeviceToHost, c->stream));
     if ((rc = fiber_attn_paged_status(c->rg_ws, c->stream))) {
-        cudaMemset(c->rg_ws, 0, c->rg_ws_bytes);
+        cudaMemsetAsync(c->rg_ws, 0, c->rg_ws_bytes, c->stream);
         return rc;
     }
     return batch_status(c);
@@ -2615,7 +2616,7 @@ extern "C" int fiber_gemm(int ggml_type, const void *d_w, int rows, int cols, co
     memset(&p, 0, sizeof(p));
     const uint8_t *w = (const uint8_t *)d_w;
     void *pad = nullptr;  // Q6_K rows re-laid at a 16-byte stride for this call
-    CK(g5_weights(nullptr, w, ggml_type, rows, cols, &w, &pad));
+    CK(g5_weights(nullptr, w, ggml_type, rows, cols, &w, st, &pad));
     if (!g5_make_map(&p.wmap, w, ggml_type, rows, cols)) {
         if (pad) cudaFree(pad);
         return set_err(FIBER_ECUDA, "fiber_gemm: cannot build the weight tensor map");

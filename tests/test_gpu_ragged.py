@@ -94,3 +94,29 @@ def test_refusals(tiny_model):
             ctx.forward_ragged(kv, slots, start, chunks)
     am, _ = ctx.forward_ragged(kv, [1], [0], [[5, 6, 7]])
     assert 0 <= am[0] < V
+
+
+def test_first_pass_does_not_depend_on_the_legacy_stream(tiny_model):
+    """Work queued on the default stream, which the context's stream does not wait for, may run beside the
+    first pass and after it: the pass's workspace is zeroed on the context's own stream."""
+    import torch
+
+    path = tiny_model("q4km")
+    hm = fb.HostModel(path)
+    rng = np.random.default_rng(11)
+    chunks = [rng.integers(1, hm.params.vocab_size, n).astype(np.int32) for n in (200, 1, 90)]
+    want = [_oracle_logits(path, c) for c in chunks]
+    a = torch.randn(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    for _ in range(3):
+        ctx = fb.Context(hm, max_seq=256, max_batch=3)
+        kv = ctx.kv(256, max_batch=3)
+        torch.cuda.synchronize()
+        b = a
+        for _ in range(40):
+            b = a @ b
+        for _ in range(2):
+            am, lg = ctx.forward_ragged(kv, [2, 0, 1], [0, 0, 0], chunks)
+            for i in range(3):
+                _check(am, lg, i, want[i])
+        torch.cuda.synchronize()
+        ctx.close()
