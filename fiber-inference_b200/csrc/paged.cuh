@@ -413,59 +413,147 @@ FDEV int attn_step_at(const AttnUnit &u, const AttnPagedParams &p, uint32_t x) {
     return d <= 0 ? 0 : min(u.steps, u.per == 1 ? d : (d + u.per - 1) / u.per);
 }
 
+// Whether x is not finite once rounded to 16 bits (half a step above the largest value is not).
+template <bool BF>
+FDEV bool attn_spoiled(float x) {
+    return !(fabsf(x) < (BF ? __uint_as_float(0x7f7f8000u) : 65520.f));
+}
+
 // One row from the definition, by one warp: only the positions the row sees are read, so
-// nothing behind a mask can reach it. Used for rows whose tile result is not finite: on
-// the tensor cores a masked position has weight 0, and 0 * inf or 0 * NaN is NaN.
+// nothing behind a mask can reach it. A score that is NaN or +inf, or none above -inf, makes
+// every weight NaN: such a row ends at the first of them. Else about 0.2 us a key, the latency of
+// one warp's instructions. Lane i takes the output's values (HD / 32) i and up.
 template <int HD, bool BF>
 static __device__ __noinline__ void attn_row_exact(const AttnPagedParams &p, const uint16_t *q, uint16_t *out, int slot,
-                                                   int g, int lo, int hi, int lane) {
+                                                   int g, uint32_t lo, uint32_t hi, int lane) {
+    constexpr int W = HD / 64;  // 32-bit words per lane
     const PagedView &c = p.kv;
-    const int mask = (1 << c.page_shift) - 1;
+    const uint32_t mask = (1u << c.page_shift) - 1;
     const int32_t *tab = c.table + (long long)slot * c.max_pages;
-    auto at = [&](int j) -> long long {  // -1: a table entry outside the pool reads as zeros
+    auto at = [&](uint32_t j) -> long long {  // -1: a table entry outside the pool reads as zeros
         const int page = tab[j >> c.page_shift];
         if (page < 0 || page >= c.n_pages) return -1;
         return (long long)page * c.page_stride + (long long)g * c.head_stride + (long long)(j & mask) * c.pos_stride;
     };
-    auto score = [&](int j) -> float {
-        const long long a = at(j);
-        if (a < 0) return 0.f;
-        float s = 0.f;
-        for (int d = 0; d < HD; d += 8) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(q + d), y = *reinterpret_cast<const uint4 *>(c.k + a + d);
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    float qf[HD / 8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = unpack2<BF>(xs[i]), h = unpack2<BF>(ys[i]);
-                s = fmaf(f.y, h.y, fmaf(f.x, h.x, s));
-            }
+    for (int d = 0; d < HD / 64; d++) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(q + 64 * d + 8 * (lane & 7));
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = unpack2<BF>(xs[i]);
+            qf[8 * d + 2 * i] = f.x;
+            qf[8 * d + 2 * i + 1] = f.y;
         }
-        return s * p.scale;
+    }
+    // The scores of 32 keys, lane i's at place a, by eight lanes to a key: 32 lanes with a key
+    // each touch 32 cache lines per load (0.28 us a key instead of 0.2).
+    auto scores = [&](long long a) -> float {
+        float mine = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const long long ak = __shfl_sync(0xffffffffu, a, 4 * i + (lane >> 3));
+            float s = 0.f;
+#pragma unroll
+            for (int d = 0; d < HD / 64; d++) {
+                uint4 y = make_uint4(0u, 0u, 0u, 0u);
+                if (ak >= 0) y = *reinterpret_cast<const uint4 *>(c.k + ak + 64 * d + 8 * (lane & 7));
+                const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const float2 h = unpack2<BF>(ys[n]);
+                    s = fmaf(qf[8 * d + 2 * n + 1], h.y, fmaf(qf[8 * d + 2 * n], h.x, s));
+                }
+            }
+            if (ak < 0) s = 0.f;
+            s += __shfl_xor_sync(0xffffffffu, s, 1);
+            s += __shfl_xor_sync(0xffffffffu, s, 2);
+            s += __shfl_xor_sync(0xffffffffu, s, 4);
+            s = __shfl_sync(0xffffffffu, s, 8 * (lane & 3));
+            if (lane >> 2 == i) mine = s;
+        }
+        return mine * p.scale;
     };
+    uint32_t *dst = reinterpret_cast<uint32_t *>(out) + W * lane;
     float m = -INFINITY;
-    for (int j = lo + lane; j < hi; j += 32) m = fmaxf(m, score(j));
+    bool nan = false;
+    for (uint32_t j0 = lo; j0 < hi && !nan; j0 += 32) {
+        const bool in = j0 + lane < hi;
+        float s = scores(in ? at(j0 + lane) : -1);
+        if (!in) s = -INFINITY;
+        nan = __any_sync(0xffffffffu, !(s < INFINITY));
+        m = fmaxf(m, s);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, o2[HD / 32];
+    if (nan || m == -INFINITY) {
 #pragma unroll
-    for (int k = 0; k < HD / 32; k++) o2[k] = 0.f;
-    for (int j0 = lo; j0 < hi; j0 += 32) {
-        const float e = j0 + lane < hi ? expf(score(j0 + lane) - m) : 0.f;
+        for (int k = 0; k < W; k++) dst[k] = 0x7fff7fffu;
+        return;
+    }
+    float l = 0.f, o2[2 * W];
+#pragma unroll
+    for (int k = 0; k < 2 * W; k++) o2[k] = 0.f;
+    for (uint32_t j0 = lo; j0 < hi; j0 += 32) {
+        const bool in = j0 + lane < hi;
+        const long long a = in ? at(j0 + lane) : -1;
+        const float s = scores(a), e = in ? expf(s - m) : 0.f;
         l += e;
-        for (int i = 0; i < min(32, hi - j0); i++) {
+#pragma unroll 8
+        for (int i = 0; i < 32; i++) {  // past the end: weight 0 and value 0
             const float w = __shfl_sync(0xffffffffu, e, i);
-            const long long a = at(j0 + i);
+            const long long av = __shfl_sync(0xffffffffu, a, i);
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(c.v + av) + W * lane;
 #pragma unroll
-            for (int k = 0; k < HD / 32; k++) {
-                const uint32_t v = a < 0 ? 0u : c.v[a + lane + 32 * k];
-                o2[k] = fmaf(w, unpack2<BF>(v).x, o2[k]);
+            for (int k = 0; k < W; k++) {
+                const float2 v = unpack2<BF>(av < 0 ? 0u : src[k]);
+                o2[2 * k] = fmaf(w, v.x, o2[2 * k]);
+                o2[2 * k + 1] = fmaf(w, v.y, o2[2 * k + 1]);
             }
         }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
-    for (int k = 0; k < HD / 32; k++) out[lane + 32 * k] = (uint16_t)pack2<BF>(o2[k] / l, 0.f);
+    for (int k = 0; k < W; k++) dst[k] = pack2<BF>(o2[2 * k] / l, o2[2 * k + 1] / l);
+}
+
+// The rows that this CTA has written (whole units, and the cut ones it has joined) and whose
+// stored result is not finite, again and exactly: on the tensor cores a masked position has
+// weight 0, and 0 * inf or 0 * NaN is NaN. By the first `warps` warps after the CTA's other work,
+// when nothing in the kernel waits any more, since how long it takes depends on the data: 64 tokens of
+// 32 heads (dim 128) over 16,384 positions, 32 rows a warp, take 0.16 ms where the first key is NaN
+// (0.08 without), 110 ms where a value is.
+template <int HD, bool BF>
+static __device__ __noinline__ void attn_exact_rows(const AttnPagedParams &p, const AttnPlan &pl, int n_cta,
+                                                    const int *joined, int ru, int bk_shift, int warps) {
+    constexpr uint32_t EXP = BF ? 0x7f80u : 0x7c00u;
+    const int cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t total = pl.prefix[p.b.n_seqs], x0 = attn_share(total, n_cta, cta), x1 = attn_share(total, n_cta, cta + 1);
+    AttnUnit u;
+    attn_unit_find(u, pl, p, ru, bk_shift, x0);
+    for (;;) {
+        const int b = u.u0 < x0 ? attn_step_at(u, p, x0) : 0, e = u.u0 + u.cost > x1 ? attn_step_at(u, p, x1) : u.steps;
+        if (u.hi > u.lo && b < e && ((b == 0 && e == u.steps) || joined[b > 0 ? 0 : 1]))
+            for (int r = warp; r < u.rows; r += warps) {
+                const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
+                const int pos = u.kv - u.nq + t;
+                if (pos < 0) continue;
+                uint16_t *out = p.out + (long long)(u.q0 + t) * p.ldo + (long long)head * HD;
+                bool bad = false;
+#pragma unroll
+                for (int k = 0; k < HD / 64; k++) {
+                    const uint32_t w = reinterpret_cast<const uint32_t *>(out)[32 * k + lane];
+                    bad |= (w & EXP) == EXP || (w >> 16 & EXP) == EXP;
+                }
+                if (__any_sync(0xffffffffu, bad))
+                    attn_row_exact<HD, BF>(p, p.q + (long long)(u.q0 + t) * p.ldq + (long long)head * HD, out, u.slot, u.g,
+                                           p.window > 0 ? max(0, pos - p.window + 1) : 0, pos + 1, lane);
+            }
+        if (u.u0 + u.cost >= x1) break;
+        attn_unit_next(u, pl, p, ru, bk_shift);
+    }
 }
 
 }  // namespace fiber

@@ -32,7 +32,8 @@ struct PrShared {
     AttnPlan plan;
     uint64_t full[8], empty[8];
     float ml[PR_WARPS][PR_ROWS][2];
-    unsigned bad;  // rows whose result is not finite
+    int bad;        // some row's result is not finite
+    int joined[2];  // this CTA has joined the cut unit at the start / at the end of its share
     int last;
     int fail;
 };
@@ -88,6 +89,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.fail = 0;
         sh.bad = 0;
+        sh.joined[0] = sh.joined[1] = 0;
     }
     if (tid == 32 * PR_WARPS) {
         pg_prefetch_map(&p.kmap);
@@ -291,7 +293,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                     const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
                     const bool sees = p0 + t >= 0;
                     a = sees ? make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (!(isfinite(a.x) && isfinite(a.y) && isfinite(a.z) && isfinite(a.w))) atomicOr(&sh.bad, 1u << r);
+                    if (attn_spoiled<BF>(a.x) || attn_spoiled<BF>(a.y) || attn_spoiled<BF>(a.z) || attn_spoiled<BF>(a.w)) sh.bad = 1;
                     *reinterpret_cast<uint2 *>(p.out + (long long)(u.q0 + t) * p.ldo + (long long)head * HD + 4 * c4) =
                         make_uint2(pack2<BF>(a.x, a.y), pack2<BF>(a.z, a.w));
                 } else {
@@ -310,7 +312,10 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                 const int ca = attn_owner(total, n_cta, attn_place(u, p, 0)), cb = attn_owner(total, n_cta, attn_place(u, p, u.steps - 1));
                 if (tid == 0) {
                     sh.last = pg_ticket(&p.tickets[ca]) == (unsigned)(cb - ca);
-                    if (sh.last) p.tickets[ca] = 0u;
+                    if (sh.last) {
+                        p.tickets[ca] = 0u;
+                        sh.joined[b > 0 ? 0 : 1] = 1;
+                    }
                 }
                 pr_bar();
                 if (sh.last) {
@@ -353,27 +358,14 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                         const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
                         const bool sees = p0 + t >= 0;
                         a = sees ? make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (!(isfinite(a.x) && isfinite(a.y) && isfinite(a.z) && isfinite(a.w))) atomicOr(&sh.bad, 1u << r);
+                        if (attn_spoiled<BF>(a.x) || attn_spoiled<BF>(a.y) || attn_spoiled<BF>(a.z) || attn_spoiled<BF>(a.w)) sh.bad = 1;
                         *reinterpret_cast<uint2 *>(p.out + (long long)(u.q0 + t) * p.ldo + (long long)head * HD + 4 * c4) =
                             make_uint2(pack2<BF>(a.x, a.y), pack2<BF>(a.z, a.w));
                     }
                     pr_bar();
                 }
             }
-            // rows whose result is not finite, again and exactly
-            const unsigned bad = *(volatile unsigned *)&sh.bad;
-            if (bad) {
-                for (int r = warp; r < u.rows; r += PR_WARPS) {
-                    if (!(bad >> r & 1)) continue;
-                    const int t = fdiv(u.row0 + r, p.by_group), head = u.g * p.group + u.row0 + r - t * p.group;
-                    attn_row_exact<HD, BF>(p, p.q + (long long)(u.q0 + t) * p.ldq + (long long)head * HD,
-                                           p.out + (long long)(u.q0 + t) * p.ldo + (long long)head * HD, u.slot, u.g,
-                                           p.window > 0 ? max(0, p0 + t - p.window + 1) : 0, p0 + t + 1, lane);
-                }
-                pr_bar();
-                if (tid == 0) sh.bad = 0;
-            }
-            pr_bar();  // sh.ml and sh.bad are reused by the next unit
+            pr_bar();  // sh.ml is reused by the next unit
         } else if (b < e) {  // no row of the unit sees a key
             for (int i = tid; i < u.rows * C4; i += 32 * PR_WARPS) {
                 const int r = i / C4, c4 = i % C4;
@@ -386,6 +378,8 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         attn_unit_next(u, sh.plan, p, PR_ROWS, PR_BK_SHIFT);
     }
     if (lane == 0 && sh.fail) *p.status = 1;
+    pr_bar();
+    if (sh.bad && !sh.fail) attn_exact_rows<HD, BF>(p, sh.plan, n_cta, sh.joined, PR_ROWS, PR_BK_SHIFT, PR_WARPS);
 }
 
 }  // namespace fiber

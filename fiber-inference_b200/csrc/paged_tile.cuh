@@ -73,6 +73,9 @@ struct PtShared {
     uint64_t join, mdone;
     PtWork work[2];
     uint32_t tmem;
+    int n_cta;      // CTAs that have work
+    int bad;        // some row's result is not finite
+    int joined[2];  // this CTA has joined the cut unit at the start / at the end of its share
     int last;
     int fail;
 };
@@ -260,6 +263,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
         pg_init(&sh.mdone, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.fail = 0;
+        sh.bad = 0;
+        sh.joined[0] = sh.joined[1] = 0;
     }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pg_saddr(&sh.tmem)) : "memory");
@@ -281,6 +286,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
     constexpr uint32_t tmem = 0;  // all 512 columns
     if (sh.tmem != tmem && tid == 0) *p.status = 2;
     const int n_cta = attn_ctas(p, total, longest), cta = blockIdx.x;
+    if (tid == 0) sh.n_cta = n_cta;
 
     // 384 threads at 168 registers: the softmax warpgroups take 224 each, the third keeps 56
     if (warp >= 8) {
@@ -638,7 +644,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
 #pragma unroll
                 for (int j = 0; j < 16; j += 8) {
 #pragma unroll
-                    for (int i2 = 0; i2 < 8; i2++) bad |= !isfinite(o[j + i2]);
+                    for (int i2 = 0; i2 < 8; i2++) bad |= attn_spoiled<BF>(o[j + i2]);
                     *reinterpret_cast<uint4 *>(dst + c + j) =
                         make_uint4(pack2<BF>(o[j], o[j + 1]), pack2<BF>(o[j + 2], o[j + 3]), pack2<BF>(o[j + 4], o[j + 5]),
                                    pack2<BF>(o[j + 6], o[j + 7]));
@@ -686,7 +692,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 pg_wait(&sh.join, nj++ & 1, &sh.fail);
                 if (tid == 0) {
                     sh.last = pg_ticket(&p.tickets[w.ca]) == (unsigned)(w.cb - w.ca);
-                    if (sh.last) p.tickets[w.ca] = 0u;
+                    if (sh.last) {
+                        p.tickets[w.ca] = 0u;
+                        sh.joined[w.slot_of & 1] = 1;
+                    }
                 }
                 __syncwarp();
                 if (lane == 0) pg_arrive(&sh.join);
@@ -732,19 +741,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                         }
                 }
             }
-            // rows whose result is not finite, again and exactly
-            unsigned again = __ballot_sync(0xffffffffu, bad);
-            while (again) {
-                const int src = __ffs(again) - 1;
-                again &= again - 1;
-                const int stok = __shfl_sync(0xffffffffu, tok, src), shead = __shfl_sync(0xffffffffu, head, src);
-                attn_row_exact<HD, BF>(p, p.q + (long long)(w.q0 + stok) * p.ldq + (long long)shead * HD,
-                                       p.out + (long long)(w.q0 + stok) * p.ldo + (long long)shead * HD, w.slot, w.g,
-                                       __shfl_sync(0xffffffffu, rlo, src), __shfl_sync(0xffffffffu, rhi, src), lane);
-            }
+            if (bad) sh.bad = 1;
             __syncwarp();
             if (lane == 0) pg_arrive(&sh.wfree[i & 1]);
         }
+        // not finite, so again: the other warps have no wait left but the CTA's last barrier
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (sh.bad && !sh.fail) attn_exact_rows<HD, BF>(p, sh.plan, sh.n_cta, sh.joined, 2 * pt_tile_rows(p.group), PT_BK_SHIFT, 8);
     }
     pt_fence_before();
     __syncthreads();

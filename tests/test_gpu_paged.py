@@ -616,3 +616,106 @@ def test_append_then_attend_equals_the_cache_class():
             p = torch.softmax(sc, 1)
             tol = 1.05 * U["f16"] * ((p @ v).abs() + p @ v.abs()) + (p @ v.abs()) * (2.0 ** -16 * 40 + 2.0 ** -15) + 2.0 ** -25 * (6 * n + 1)
             assert ((out[at:at + n, head * 64:(head + 1) * 64].double() - p @ v).abs() <= tol).all()
+
+
+# ---- rows that are computed again ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,lens,window", [
+    (4, 1, [(3, 3000)], 0), (8, 1, [(40, 3000)], 0), (4, 1, [(3, 3000), (2, 700)], 500),
+    (8, 2, [(300, 2500), (1, 60), (20, 900)], 0), (6, 6, [(2, 40)] * 90, 0)], ids=str)
+def test_attn_rows_computed_again_in_cut_and_whole_units(heads, kv_heads, lens, window, dim, dtype):
+    """The last token's value is infinite: every earlier row of its tile is computed again, by whichever
+    CTA wrote it, and only the last token's row sees it."""
+    torch = torch_()
+    s = Setup(lens, heads, kv_heads, dim, dtype, 16, window=window, seed=31)
+    last = []
+    for q, (n, kv) in enumerate(lens):
+        s.v[int(s.table[s.order[q], (kv - 1) // 16]), :, (kv - 1) % 16] = float("inf")
+        last.append(s.starts[q] + n - 1)
+    s.dv.copy_(s.v)
+    s.attend()
+    fb.attn_paged_status(s.ws.data_ptr())
+    first = s.out.clone()
+    for _ in range(3):
+        s.out.fill_(7.0)
+        s.attend()
+        assert torch.equal(s.out, first)
+    got = first[:s.n, :heads * dim].double().reshape(s.n, heads, dim)
+    assert (got[last] == float("inf")).all()
+    G, u = heads // kv_heads, U[dtype]
+    for q, (n, kv) in enumerate(lens):
+        k, v = s.cached(s.k, q).cuda(), s.cached(s.v, q).cuda()
+        v[kv - 1] = 0.0
+        pos = torch.arange(n - 1, device="cuda")[:, None] + kv - n
+        key = torch.arange(kv, device="cuda")[None]
+        seen = (key <= pos) & ((key > pos - window) if window else True)
+        for h in range(heads):
+            x = s.dq[s.starts[q]:s.starts[q] + n - 1, h * dim:(h + 1) * dim].double()
+            if n == 1:
+                continue
+            big = float((x.abs() @ k[:, h // G].abs().T).max()) * s.scale
+            p = torch.softmax(torch.where(seen, x @ k[:, h // G].T * s.scale, -math.inf), 1)
+            o, w = p @ v[:, h // G], p @ v[:, h // G].abs()
+            tol = 1.05 * u * (o.abs() + w) + w * (2.0 ** -16 * big + 2.0 ** -15) + 2.0 ** -25 * (kv * float(v.abs().max()) + 1)
+            err = (got[s.starts[q]:s.starts[q] + n - 1, h] - o).abs()
+            assert (err <= tol).all(), (q, h, float((err / tol).max()))
+
+
+def test_attn_long_rows_computed_again_hold_nobody_up():
+    """256 rows over 160,000 positions of which the first holds a NaN value that they see, in front of clean
+    units of the same CTA: the clean rows keep their bits and no wait gives up."""
+    torch = torch_()
+    P, KV, G, D, kv, n = 256, 8, 16, 64, 160_000, 16  # a unit is 16 tokens of 16 heads
+    H, pages = KV * G, -(-kv // P)
+    n_seqs = -(-2 * torch.cuda.get_device_properties(0).multi_processor_count // KV)  # two units a CTA
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(17)
+    # every sequence reads the same pages, the first one with a first page of its own
+    pools = [torch.randn(pages + 1, KV, P, D, generator=gen, device="cuda").bfloat16() for _ in range(2)]
+    for p in pools:
+        p[pages] = p[0]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(n_seqs, 1)
+    table[0, 0] = pages
+    q = torch.randn(n_seqs * n, H * D, generator=gen, device="cuda").bfloat16()
+    out = torch.zeros_like(q)
+    start = torch.arange(n_seqs + 1, dtype=torch.int32, device="cuda") * n
+    lens = torch.full((n_seqs,), kv, dtype=torch.int32, device="cuda")
+    view = fb.PagedKV(pools[0].data_ptr(), pools[1].data_ptr(), table.data_ptr(), n_slots=n_seqs, max_pages=pages,
+                      n_pages=pages + 1, page_size=P, n_kv_heads=KV, head_dim=D, dtype=30)
+    batch = fb.RaggedBatch(start.data_ptr(), lens.data_ptr(), n_seqs=n_seqs, n_tokens=n_seqs * n, max_q=n)
+    ws = torch.zeros(fb.attn_paged_workspace(view, batch, H), dtype=torch.uint8, device="cuda")
+
+    def attend():
+        fb.attn_paged(view, batch, q.data_ptr(), out.data_ptr(), n_heads=H, ldq=H * D, ldo=H * D, scale=0.125,
+                      ws=ws.data_ptr(), ws_bytes=ws.numel())
+        fb.attn_paged_status(ws.data_ptr())
+        return out.clone()
+
+    clean = attend()
+    assert torch.isfinite(clean).all()
+    pools[1][pages, 0, 0, 3] = float("nan")  # KV head 0 of the first sequence
+    got = attend()
+    hit = torch.zeros(n_seqs * n, H, dtype=torch.bool, device="cuda")
+    hit[:n, :G] = True
+    got, clean = got.reshape(-1, H, D), clean.reshape(-1, H, D)
+    assert torch.equal(got[~hit], clean[~hit])
+    assert torch.isnan(got[:n, :G, 3]).all()
+    others = [d for d in range(D) if d != 3]
+    k, v = (p[table[0].long(), 0].reshape(-1, D)[:kv].double() for p in pools)
+    v[0, 3] = 0.0
+    seen = torch.arange(kv, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None] + kv - n
+    for h in range(G):
+        x = q[:n, h * D:(h + 1) * D].double()
+        big = float((x.abs() @ k.abs().T).max()) * 0.125
+        p = torch.softmax(torch.where(seen, x @ k.T * 0.125, -math.inf), 1)
+        o, w = p @ v, p @ v.abs()
+        tol = 1.05 * U["bf16"] * (o.abs() + w) + w * (2.0 ** -16 * big + 2.0 ** -15)
+        assert ((got[:n, h].double() - o).abs() <= tol)[:, others].all()
+    # a key that is NaN: the rows that see it are NaN at once
+    pools[1][pages, 0, 0, 3] = 0.0
+    pools[0][pages, 0, 0, 3] = float("nan")
+    got = attend().reshape(-1, H, D)
+    assert torch.isnan(got[:n, :G]).all() and torch.equal(got[~hit], clean[~hit])
