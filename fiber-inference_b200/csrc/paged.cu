@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "fiber_cuda.h"
 #include "fiber_paged.h"
@@ -43,6 +44,8 @@ int sm_count() {
     }
     return cache[dev];
 }
+
+std::atomic<int> drill{0};
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -328,6 +331,8 @@ extern "C" int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t 
     p.cost = shape.tile ? PT_COST : PR_COST;
     p.scale = scale;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+    p.drill = drill.load();
+    p.wait_limit = p.drill ? PG_DRILL_CYCLES : PG_WAIT_CYCLES;
     uint8_t *ws = (uint8_t *)d_ws;
     p.status = (int *)ws;
     p.tickets = (unsigned int *)(ws + WS_TICKETS);
@@ -351,6 +356,11 @@ extern "C" int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t 
             e = hd == 64 ? launch_attn<64, true>(p, shape, st) : launch_attn<128, true>(p, shape, st);
         if (e != cudaSuccess) return fail(FIBER_ECUDA, "%s: %s", fn, cudaGetErrorString(e));
     }
+    return FIBER_OK;
+}
+
+extern "C" int fiber_attn_paged_drill(int on) {
+    drill.store(on != 0);
     return FIBER_OK;
 }
 

@@ -104,7 +104,8 @@ FDEV uint32_t pack2(float a, float b) {  // a in the low half
 
 // ---- mbarriers and TMA -------------------------------------------------------------------
 
-constexpr long long PG_WAIT_CYCLES = 4000000000ll;  // about 2 s
+constexpr long long PG_WAIT_CYCLES = 4000000000ll;   // about 2 s
+constexpr long long PG_DRILL_CYCLES = 1000000ll;      // about 0.5 ms: the limit in a drill
 
 FDEV uint32_t pg_saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 FDEV void pg_init(uint64_t *bar, int count) {
@@ -120,23 +121,31 @@ FDEV bool pg_try(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 // Waits for the phase of that parity; gives up when another thread of the CTA has
-// (*fail), or after PG_WAIT_CYCLES (then sets *fail). The clock is looked at once in 256
-// tries only: a timer read before the first retry delayed every hand-over that was not
-// ready at once.
-FDEV bool pg_wait(uint64_t *bar, uint32_t parity, volatile int *fail) {
+// (*fail), or after `limit` cycles (then sets *fail). The clock is looked at once in 256 tries
+// only: a timer read before the first retry delayed every hand-over that was not ready at once.
+FDEV bool pg_wait(uint64_t *bar, uint32_t parity, volatile int *fail, long long limit) {
     long long t0 = 0;
     for (uint32_t n = 0; !pg_try(bar, parity); n++) {
         if (n & 255) continue;
         if (fail && *fail) return false;
         const long long now = clock64();
         if (n == 0) t0 = now;
-        if (now - t0 > PG_WAIT_CYCLES) {
+        if (now - t0 > limit) {
             if (fail) *fail = 1;
             return false;
         }
     }
     return true;
 }
+// The same by a whole warp, whose lanes may give up at different tries: they meet again
+// before the warp-wide instructions that follow.
+FDEV void pg_wait_warp(uint64_t *bar, uint32_t parity, volatile int *fail, long long limit) {
+    pg_wait(bar, parity, fail, limit);
+    __syncwarp();
+}
+// Waits for copies or products of this CTA that are in flight when it gives up or ends: always
+// with the full limit.
+FDEV void pg_drain(uint64_t *bar, uint32_t parity) { pg_wait(bar, parity, nullptr, PG_WAIT_CYCLES); }
 FDEV void pg_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pg_saddr(bar)) : "memory");
 }
@@ -192,6 +201,8 @@ struct AttnPagedParams {
     int window;
     float scale, scale_log2;  // scale * log2(e): scores in powers of two
     AttnCost cost;
+    long long wait_limit;     // cycles after which a wait gives up
+    int drill;                // 1: no ring stage is ever free again, so that waits run out; else 0
     int *status;              // workspace: set to 1 when a wait gave up
     unsigned int *tickets;    // one per CTA, zero between calls
     float *part_ml;           // [2 * n_cta][rows][2]: running maximum (powers of two) and sum

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
     if (tid == 0) {
         for (int s = 0; s < NST; s++) {
             pg_init(&sh.full[s], 1);
-            pg_init(&sh.empty[s], PR_WARPS);
+            pg_init(&sh.empty[s], PR_WARPS + p.drill);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.fail = 0;
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
                     int page = p.kv.n_pages;  // outside the tensor: reads as zeros
                     if (lane < n_box && lp < used) page = tab[lp];
                     const int st = it % NST;
-                    if (it >= NST) ok = pg_wait(&sh.empty[st], (it / NST - 1) & 1, &sh.fail);
+                    if (it >= NST) ok = pg_wait(&sh.empty[st], (it / NST - 1) & 1, &sh.fail, p.wait_limit);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (lane == 0) pg_expect_tx(&sh.full[st], SB);
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         // every copy has landed before the CTA exits
         if (lane == 0)
             for (uint32_t s = 0; s < NST && s < it; s++)
-                pg_wait(&sh.full[s], (s + (it - 1 - s) / NST * NST) / NST & 1, nullptr);
+                pg_drain(&sh.full[s], (s + (it - 1 - s) / NST * NST) / NST & 1);
         if (lane == 0 && sh.fail) *p.status = 1;
         return;
     }
@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         if (any && b < e) {
             for (int k = b; k < e; k++, it++) {
                 st = it % NST;
-                pg_wait(&sh.full[st], (it / NST) & 1, &sh.fail);  // after a timeout: runs through, status says so
+                // after a timeout: runs through, status says so
+                pg_wait_warp(&sh.full[st], (it / NST) & 1, &sh.fail, p.wait_limit);
                 uint8_t *kt = ring + st * SB, *vt = kt + SB / 2;
                 const int key0 = (((u.lo >> PR_BK_SHIFT) + k) << PR_BK_SHIFT) + 16 * warp;
                 const bool edge = key0 < all_lo || key0 + 16 > all_hi;

@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
     if (tid == 0) {
         for (int s = 0; s < NST; s++) {
             pg_init(&sh.kvfull[s], 1);
-            pg_init(&sh.kvfree[s], 2);
+            pg_init(&sh.kvfree[s], 2 + p.drill);
         }
         pg_init(&sh.qfull, 1);
         pg_init(&sh.qfree, 2);
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                     if (!end) attn_unit_next(u, sh.plan, p, ru, PT_BK_SHIFT);
                     continue;
                 }
-                bool ok = i < 2 || pg_wait(&sh.wfree[i & 1], ((i >> 1) - 1) & 1, &sh.fail);
+                bool ok = i < 2 || pg_wait(&sh.wfree[i & 1], ((i >> 1) - 1) & 1, &sh.fail, p.wait_limit);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 PtWork &w = sh.work[i & 1];
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
             const uint32_t dst0 = half * (128 * 128) + rb * box_rows * 128;
             uint32_t it = 0, nq = 0;  // K / V tiles and Q pairs issued
             for (uint32_t i = 0;; i++) {
-                bool ok = pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail);
+                bool ok = pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail, p.wait_limit);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const PtWork &w = sh.work[i & 1];
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
 #pragma unroll
                         for (int v = 0; v < 2; v++, it++) {
                             const int st = it % NST;
-                            if (it >= NST) ok = pg_wait(&sh.kvfree[st], (it / NST - 1) & 1, &sh.fail);
+                            if (it >= NST) ok = pg_wait(&sh.kvfree[st], (it / NST - 1) & 1, &sh.fail, p.wait_limit);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
                             if (lane == 0) pg_expect_tx(&sh.kvfull[st], TB);
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                         }
                         if (!ok) break;
                         if (k == w.b) {  // the queries' buffer is free last: K and V of the first step go before
-                            if (nq > 0) ok = pg_wait(&sh.qfree, (nq - 1) & 1, &sh.fail);
+                            if (nq > 0) ok = pg_wait(&sh.qfree, (nq - 1) & 1, &sh.fail, p.wait_limit);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
                             if (lane == 0) {
@@ -401,8 +401,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
             }
             if (lane == 0) {  // every copy has landed before the CTA exits
                 for (uint32_t s = 0; s < NST && s < it; s++)
-                    pg_wait(&sh.kvfull[s], (s + (it - 1 - s) / NST * NST) / NST & 1, nullptr);
-                if (nq > 0) pg_wait(&sh.qfull, (nq - 1) & 1, nullptr);
+                    pg_drain(&sh.kvfull[s], (s + (it - 1 - s) / NST * NST) / NST & 1);
+                if (nq > 0) pg_drain(&sh.qfull, (nq - 1) & 1);
             }
         } else if (cta < n_cta && (warp == 8 || warp == 11)) {
             // ---- MMA issuer of tile t
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 if (last) pt_commit(me, &sh.odone[t]);
             };
             for (uint32_t i = 0;; i++) {
-                bool ok = pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail);
+                bool ok = pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail, p.wait_limit);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const PtWork &w = sh.work[i & 1];
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 if (lane == 0) pg_arrive(&sh.wfree[i & 1]);
                 if (!run) continue;
                 auto on = [&](int j) { return j >= ab && j < ae; };
-                ok = pg_wait(&sh.qfull, nq & 1, &sh.fail) && pg_wait(&sh.kvfull[st], ph, &sh.fail);
+                ok = pg_wait(&sh.qfull, nq & 1, &sh.fail, p.wait_limit) && pg_wait(&sh.kvfull[st], ph, &sh.fail, p.wait_limit);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 nq++;
@@ -460,12 +460,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 for (int k = b; k < e; k++) {
                     const bool more = k + 1 < e;
                     const int vst = st;
-                    ok = pg_wait(&sh.kvfull[st], ph, &sh.fail);
+                    ok = pg_wait(&sh.kvfull[st], ph, &sh.fail, p.wait_limit);
                     next();  // now the next step's K tile
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         if (on(2 * k + h)) {
-                            ok = ok && pg_wait(&sh.pready[t][h], np >> h & 1, &sh.fail);
+                            ok = ok && pg_wait(&sh.pready[t][h], np >> h & 1, &sh.fail, p.wait_limit);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
                             np ^= 1u << h;
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                             values(h, vst, 2 * k + h == ab, 2 * k + h + 1 == ae);
                         }
                         if (h == 1) pt_commit(me, &sh.kvfree[vst]);
-                        if (more && h == 0) ok = ok && pg_wait(&sh.kvfull[st], ph, &sh.fail);
+                        if (more && h == 0) ok = ok && pg_wait(&sh.kvfull[st], ph, &sh.fail, p.wait_limit);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         if (more && on(2 * k + 2 + h)) scores(h);
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 if (!ok) break;
             }
             pt_commit(me, &sh.mdone);  // every product has finished before tensor memory is released
-            pg_wait(&sh.mdone, 0, nullptr);
+            pg_drain(&sh.mdone, 0);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
         const uint64_t scale2 = pt_two(p.scale_log2, p.scale_log2);
         uint32_t it = 0, ns = 0, npv = 0, no = 0, nj = 0;  // ns: parity of sfull[t][h] in bit h; npv: products of this tile
         for (uint32_t i = 0; cta < n_cta; i++) {
-            if (!__all_sync(0xffffffffu, pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail))) break;
+            if (!__all_sync(0xffffffffu, pg_wait(&sh.wfull[i & 1], (i >> 1) & 1, &sh.fail, p.wait_limit))) break;
             const PtWork &w = sh.work[i & 1];
             const int mode = w.mode;
             if (mode == PT_END) break;
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
             float m = -INFINITY, l = 0.f;
             auto await = [&](int j) {  // the scores of half step j are there
                 const int h = j & 1;
-                pg_wait(&sh.sfull[t][h], ns >> h & 1, &sh.fail);
+                pg_wait_warp(&sh.sfull[t][h], ns >> h & 1, &sh.fail, p.wait_limit);
                 ns ^= 1u << h;
                 pt_fence_after();
             };
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                     // Each tile clears them before its own product: the tiles' products do not
                     // wait for one another (zeros over the other tile's zeros change nothing).
                     const uint32_t vi = it + 2 * ((j >> 1) - w.b) + 1;
-                    pg_wait(&sh.kvfull[vi % NST], vi / NST & 1, &sh.fail);
+                    pg_wait_warp(&sh.kvfull[vi % NST], vi / NST & 1, &sh.fail, p.wait_limit);
                     if (tile0 + row < w.lo || tile0 + row >= w.hi)
 #pragma unroll 1
                         for (int c = 0; c < 8 * HALVES; c++)  // pieces rotated by the row: eight rows on eight banks
@@ -584,8 +584,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                     m = mn;
                     l *= f;
                     if (j > ab) {
-                        pg_wait(&sh.pvdone[t], (npv - 1) & 1, &sh.fail);  // the half before is in O (the one before
-                        pt_fence_after();                                 // that had finished when v's scores did)
+                        // the half before is in O (the one before that had finished when v's scores did)
+                        pg_wait_warp(&sh.pvdone[t], (npv - 1) & 1, &sh.fail, p.wait_limit);
+                        pt_fence_after();
 #pragma unroll
                         for (int c = 0; c < HD; c += 16) {
                             float o[16];
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
             if (w.ae[0] > w.ab[0] || w.ae[1] > w.ab[1]) it += 2 * (w.e - w.b);
             const bool did = ae > ab;
             if (did) {
-                pg_wait(&sh.odone[t], no++ & 1, &sh.fail);
+                pg_wait_warp(&sh.odone[t], no++ & 1, &sh.fail, p.wait_limit);
                 pt_fence_after();
             }
             const int tok = fdiv(row0 + row, p.by_group), head = w.g * p.group + row0 + row - tok * p.group;
@@ -689,7 +690,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 }
                 __syncwarp();
                 if (lane == 0) pg_arrive(&sh.join);
-                pg_wait(&sh.join, nj++ & 1, &sh.fail);
+                pg_wait_warp(&sh.join, nj++ & 1, &sh.fail, p.wait_limit);
                 if (tid == 0) {
                     sh.last = pg_ticket(&p.tickets[w.ca]) == (unsigned)(w.cb - w.ca);
                     if (sh.last) {
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
                 }
                 __syncwarp();
                 if (lane == 0) pg_arrive(&sh.join);
-                pg_wait(&sh.join, nj++ & 1, &sh.fail);
+                pg_wait_warp(&sh.join, nj++ & 1, &sh.fail, p.wait_limit);
                 if (sh.last && !idle) {
                     const int c0 = w.ca, c1 = w.cb;
                     float M = -INFINITY, L = 0.f;

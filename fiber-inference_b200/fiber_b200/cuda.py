@@ -32,7 +32,7 @@ EXPORTED = [
     "kv_cache_free", "kv_cache_write", "kv_cache_read", "fiber_gemv_argmax_noalloc", "fiber_prefill_slot",
     "fiber_decode_greedy_batch", "fiber_sample", "fiber_decode_sample", "fiber_tp_collective", "fiber_set_max_batch",
     "fiber_step_ring_bytes", "fiber_forward_ragged", "fiber_kv_view", "fiber_kv_append", "fiber_attn_paged",
-    "fiber_attn_paged_workspace", "fiber_attn_paged_status",
+    "fiber_attn_paged_workspace", "fiber_attn_paged_status", "fiber_attn_paged_drill",
 ]
 
 

@@ -12,7 +12,7 @@ import ctypes as C
 from .cuda import FiberError, _check, _stream_ptr, cuda_lib
 
 __all__ = ["GGML_BF16", "PagedKV", "RaggedBatch", "Rope", "kv_view", "kv_append", "attn_paged", "attn_paged_workspace",
-           "attn_paged_status"]
+           "attn_paged_status", "attn_paged_drill"]
 
 GGML_BF16 = 30
 
@@ -72,6 +72,7 @@ def _paged_lib() -> C.CDLL:
         L.fiber_attn_paged.argtypes = [V, B, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_int,
                                        C.c_void_p, C.c_size_t, C.c_void_p]
         L.fiber_attn_paged_status.argtypes = [C.c_void_p, C.c_void_p]
+        L.fiber_attn_paged_drill.argtypes = [C.c_int]
         _lib = L
     return _lib
 
@@ -115,3 +116,8 @@ def attn_paged(kv: PagedKV, batch: RaggedBatch, q: int, out: int, *, n_heads: in
 def attn_paged_status(ws: int, stream=None):
     """Waits for the stream; raises if a bounded wait inside an attn_paged call gave up."""
     _check(_paged_lib().fiber_attn_paged_status(ws, _stream_ptr(stream)), "fiber_attn_paged_status")
+
+
+def attn_paged_drill(on: bool):
+    """fiber_attn_paged_drill: while on, waits inside later attn_paged calls run out."""
+    _check(_paged_lib().fiber_attn_paged_drill(int(on)), "fiber_attn_paged_drill")

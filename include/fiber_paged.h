@@ -101,6 +101,12 @@ int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t *batch, con
  * this workspace gave up (FIBER_ETIMEOUT; zero-fill the workspace before using it again). */
 int fiber_attn_paged_status(const void *d_ws, void *stream);
 
+/* Drill, for a program to try out how it takes a call whose waits give up: while `on`, the kernels of
+ * the whole process's later calls never reuse a stage of their shared-memory rings, and wait 1e6
+ * cycles (about 0.5 ms) instead of 4e9 (about 2 s). A call long enough to need a stage again (about
+ * 1,000 positions per SM) ends with FIBER_ETIMEOUT as its status. */
+int fiber_attn_paged_drill(int on);
+
 #ifdef __cplusplus
 }
 #endif

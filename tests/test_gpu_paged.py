@@ -719,3 +719,33 @@ def test_attn_long_rows_computed_again_hold_nobody_up():
     pools[0][pages, 0, 0, 3] = float("nan")
     got = attend().reshape(-1, H, D)
     assert torch.isnan(got[:n, :G]).all() and torch.equal(got[~hit], clean[~hit])
+
+
+# ---- waits that give up ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("nq", [1, 40], ids=["rows", "tile"])
+def test_attn_waits_that_give_up_are_reported_and_the_workspace_serves_again(nq, dim):
+    torch = torch_()
+    lens = [(nq, 3000)] * 64 + [(1, 70)]  # some 2,000 positions and more per SM, one head each
+    s = Setup(lens, 8, 2, dim, "f16", 64, seed=41)
+    s.attend()
+    fb.attn_paged_status(s.ws.data_ptr())
+    first = s.out.clone()
+    assert torch.isfinite(first).all()
+    fb.attn_paged_drill(True)
+    try:
+        s.attend()
+        with pytest.raises(fb.FiberError, match="gave up"):
+            fb.attn_paged_status(s.ws.data_ptr())
+        with pytest.raises(fb.FiberError, match="status -5"):  # it stays until the workspace is cleared
+            fb.attn_paged_status(s.ws.data_ptr())
+    finally:
+        fb.attn_paged_drill(False)
+    s.ws.zero_()
+    for _ in range(2):
+        s.out.fill_(7.0)
+        s.attend()
+        fb.attn_paged_status(s.ws.data_ptr())
+        assert torch.equal(s.out, first)
