@@ -2239,11 +2239,12 @@ extern "C" int fiber_forward_ragged(fiber_ctx_t *c, kv_cache_t *kv, int n_seqs, 
     if (argmax_or_null)
         CK(cudaMemcpyAsync(argmax_or_null, c->bt_arg, (size_t)n_seqs * 4, cudaMemcpyDeviceToHost, c->stream));
     CK(cudaMemcpyAsync(c->h_io, c->io, sizeof(StepIO), cudaMemcpyDeviceToHost, c->stream));
-    if ((rc = fiber_attn_paged_status(c->rg_ws, c->stream))) {
-        cudaMemsetAsync(c->rg_ws, 0, c->rg_ws_bytes, c->stream);
-        return rc;
-    }
-    return batch_status(c);
+    rc = fiber_attn_paged_status(c->rg_ws, c->stream);
+    if (rc && rc != FIBER_ETIMEOUT) return rc;
+    const int other = batch_status(c);  // clears what the GEMMs' waits may have left, also where the attention gave up
+    if (rc == FIBER_OK) return other;
+    CK(cudaMemsetAsync(c->rg_ws, 0, c->rg_ws_bytes, c->stream));
+    return set_err(rc, "ragged pass: a wait inside the attention gave up");
 }
 
 extern "C" int fiber_decode_greedy_batch(fiber_ctx_t *c, kv_cache_t *kv, const int32_t *first_tokens,

@@ -120,3 +120,29 @@ def test_first_pass_does_not_depend_on_the_legacy_stream(tiny_model):
                 _check(am, lg, i, want[i])
         torch.cuda.synchronize()
         ctx.close()
+
+
+def test_a_pass_whose_waits_give_up_says_so_and_the_next_one_is_right(tiny_model):
+    """64 single tokens at position 1,990 of a zero cache: long enough for the drill to end the attention."""
+    hm = fb.HostModel(tiny_model("q4km"))
+    ctx = fb.Context(hm, max_seq=2048, max_batch=64)
+    kv = ctx.kv(2048, max_batch=64)
+    prompt = np.random.default_rng(3).integers(1, hm.params.vocab_size, 40).astype(np.int32)
+    greedy = ctx.prefill(kv, prompt, slot=0)
+    toks = np.random.default_rng(2).integers(1, hm.params.vocab_size, 64).astype(np.int32)
+
+    def step():
+        return ctx.forward_ragged(kv, list(range(64)), [1990] * 64, [[t] for t in toks])
+
+    am, lg = step()
+    assert np.isfinite(lg).all()
+    fb.attn_paged_drill(True)
+    try:
+        with pytest.raises(fb.FiberError, match="status -5"):
+            step()
+    finally:
+        fb.attn_paged_drill(False)
+    for _ in range(2):
+        am2, lg2 = step()
+        assert np.array_equal(am2, am) and np.array_equal(lg2, lg)
+    assert ctx.prefill(kv, prompt, slot=0) == greedy
