@@ -56,8 +56,10 @@ static int set_err(int code, const char *fmt, ...) {
 #define CK(call)                                                                                  \
     do {                                                                                          \
         cudaError_t e_ = (call);                                                                  \
-        if (e_ != cudaSuccess)                                                                    \
+        if (e_ != cudaSuccess) {                                                                  \
+            cudaGetLastError(); /* reported here, not by the next launch's check */               \
             return set_err(FIBER_ECUDA, "%s:%d %s: %s", __FILE__, __LINE__, #call, cudaGetErrorString(e_)); \
+        }                                                                                         \
     } while (0)
 
 extern "C" const char *fiber_last_error(void) { return g_err; }
@@ -2155,9 +2157,11 @@ static int forward_batch(gpu_context *c, kv_cache_t *kv, const int32_t *tokens, 
 
 // ---- ragged pass: prompt chunks and single tokens of several slots ---------------------
 
+// Buffers of the ragged pass, made on first use: rg_ws_bytes is set when all are there, and
+// a call after one that failed goes on with what it left.
 static int rg_alloc(gpu_context *c, const kv_cache_t *kv) {
     int rc = pf_alloc(c);
-    if (rc || c->rg_ws) return rc;
+    if (rc || c->rg_ws_bytes) return rc;
     fiber_kv_view_t view;
     if ((rc = fiber_kv_view(kv, 0, &view))) return rc;
     const fiber_ragged_t most = {c->max_batch, PF_CHUNK, PF_CHUNK, (const int32_t *)kv->page_table, kv->page_table, nullptr};
@@ -2166,10 +2170,10 @@ static int rg_alloc(gpu_context *c, const kv_cache_t *kv) {
                                   fiber_attn_paged_workspace(&view, &least, c->nh_l));
     if (!bytes) return FIBER_EUNSUPPORTED;  // fiber_last_error() has the reason
     const size_t row = (size_t)c->nh_l * c->p.head_dim * 2;
-    CK(cudaMalloc(&c->rg_meta, (3 * (size_t)c->max_batch + 1) * 4));
-    CK(cudaMalloc(&c->rg_q, PF_CHUNK * row));
-    CK(cudaMalloc(&c->rg_att, PF_CHUNK * row));
-    CK(cudaMalloc(&c->rg_ws, bytes));
+    if (!c->rg_meta) CK(cudaMalloc(&c->rg_meta, (3 * (size_t)c->max_batch + 1) * 4));
+    if (!c->rg_q) CK(cudaMalloc(&c->rg_q, PF_CHUNK * row));
+    if (!c->rg_att) CK(cudaMalloc(&c->rg_att, PF_CHUNK * row));
+    if (!c->rg_ws) CK(cudaMalloc(&c->rg_ws, bytes));
     CK(cudaMemsetAsync(c->rg_ws, 0, bytes, c->stream));
     c->rg_ws_bytes = bytes;
     return FIBER_OK;
