@@ -749,3 +749,39 @@ def test_attn_waits_that_give_up_are_reported_and_the_workspace_serves_again(nq,
         s.attend()
         fb.attn_paged_status(s.ws.data_ptr())
         assert torch.equal(s.out, first)
+
+
+# ---- many small weights ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("group", [1, 24], ids=["rows", "tile"])
+@pytest.mark.parametrize("at", [0, 70_001, 131_071])
+@pytest.mark.parametrize("below", [17.5, 18.75])
+def test_attn_small_weights_of_many_keys_are_not_lost(below, at, group):
+    """One key, of value 0, `below` nats above 131,071 others, of value 1: each weighs less than 2^-25 of it,
+    together 0.1 to 0.3 percent. Beyond the general bound's terms a weight may be off by 2^-31 of the largest.
+    128 sequences of 3 KV heads share the pages: more units than CTAs, so that most are not cut."""
+    torch = torch_()
+    kv, P, D, KV, S = 131_072, 256, 64, 3, 128
+    H = KV * group
+    k = torch.zeros(kv // P, KV, P, D, dtype=torch.float16, device="cuda")
+    v = torch.ones_like(k)
+    k[at // P, :, at % P, 0] = 16.0
+    v[at // P, :, at % P] = 0.0
+    q = torch.zeros(S, H * D, dtype=torch.float16, device="cuda")
+    q[:, ::D] = below / 2  # scores 16 * below / 2 * 0.125 = below, and 0: exact
+    out = torch.zeros_like(q)
+    start = torch.arange(S + 1, dtype=torch.int32, device="cuda")
+    lens = torch.full((S,), kv, dtype=torch.int32, device="cuda")
+    table = torch.arange(kv // P, dtype=torch.int32, device="cuda").repeat(S, 1)
+    view = fb.PagedKV(k.data_ptr(), v.data_ptr(), table.data_ptr(), n_slots=S, max_pages=kv // P, n_pages=kv // P,
+                      page_size=P, n_kv_heads=KV, head_dim=D)
+    batch = fb.RaggedBatch(start.data_ptr(), lens.data_ptr(), n_seqs=S, n_tokens=S, max_q=1)
+    ws = torch.zeros(fb.attn_paged_workspace(view, batch, H), dtype=torch.uint8, device="cuda")
+    fb.attn_paged(view, batch, q.data_ptr(), out.data_ptr(), n_heads=H, ldq=H * D, ldo=H * D, scale=0.125,
+                  ws=ws.data_ptr(), ws_bytes=ws.numel())
+    fb.attn_paged_status(ws.data_ptr())
+    small = (kv - 1) * math.exp(-below)
+    want = small / (1.0 + small)
+    tol = 1.05 * U["f16"] * 2 * want + want * (2.0 ** -16 * below + 2.0 ** -15) + 2.0 ** -31 * kv
+    assert float((out.double() - want).abs().max()) <= tol
