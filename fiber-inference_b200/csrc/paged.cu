@@ -177,8 +177,12 @@ struct AttnShape {
     int n_cta, rows;  // CTAs of a launch, rows of a unit's state
 };
 
+bool tile_kernel(const fiber_kv_view_t *kv, const fiber_ragged_t *b, int n_heads) {
+    return b->max_q * (long long)(n_heads / kv->n_kv_heads) > PR_ROWS;
+}
+
 AttnShape attn_shape(const fiber_kv_view_t *kv, const fiber_ragged_t *b, int n_heads) {
-    if (b->max_q * (long long)(n_heads / kv->n_kv_heads) > PR_ROWS)
+    if (tile_kernel(kv, b, n_heads))
         return {true, std::min(sm_count(), WS_MAX_CTAS), 2 * PT_ROWS};
     return {false, std::min(sm_count() * PR_CTAS_PER_SM, WS_MAX_CTAS), PR_ROWS};
 }
@@ -214,9 +218,15 @@ int check_attn(const char *fn, const fiber_kv_view_t *kv, const fiber_ragged_t *
     if (b->n_tokens && b->max_q < 1) return fail(FIBER_EARG, "%s: max_q %d", fn, b->max_q);
     if (n_heads <= 0 || n_heads % kv->n_kv_heads || n_heads / kv->n_kv_heads > 128)
         return fail(FIBER_EARG, "%s: %d query heads over %d KV heads", fn, n_heads, kv->n_kv_heads);
-    // the cost of a launch is counted in 32 bits
-    const double rows = (double)b->n_tokens * (n_heads / kv->n_kv_heads) / PR_ROWS + b->n_seqs;
-    if (rows * kv->n_kv_heads * ((double)kv->max_pages * kv->page_size / PR_BK + 8) > 1e9)
+    // Rows of a sequence, and the cost of a launch (attn_plan_build), are counted in 32 bits: at
+    // most this many units, none of more steps than the table has room for.
+    const int group = n_heads / kv->n_kv_heads;
+    const bool tile = tile_kernel(kv, b, n_heads);
+    const double rows = (double)b->n_tokens * group, ru = tile ? 2 * pt_tile_rows(group) : PR_ROWS;
+    const double units = (rows / ru + std::min(b->n_seqs, PG_MAX_SEQS)) * kv->n_kv_heads;
+    const AttnCost cost = tile ? PT_COST : PR_COST;
+    const double steps = (double)kv->max_pages * kv->page_size / (tile ? PT_BK : PR_BK) + 1;
+    if (rows > 2147483647. - 2 * PT_ROWS || units * (cost.unit + cost.full * steps) > 4294967295.)
         return fail(FIBER_EARG, "%s: batch too large (%d tokens over %d positions)", fn, b->n_tokens,
                     kv->max_pages * kv->page_size);
     return FIBER_OK;

@@ -51,7 +51,8 @@ int fiber_kv_view(const kv_cache_t *kv, int layer, fiber_kv_view_t *out);
  * cache slot slot[s] (slot null: slot s); its token i sits at position
  * kv_len[s] - (q_start[s + 1] - q_start[s]) + i. Tokens at negative positions are not
  * in the cache: they are not stored and attend to nothing (zero output); so do all
- * tokens of a sequence whose slot or kv_len lies outside the table. */
+ * tokens of a sequence whose slot or kv_len lies outside the table. Rows before q_start[0]
+ * and from q_start[n_seqs] on belong to no sequence: neither operator writes them. */
 typedef struct {
     int n_seqs, n_tokens; /* n_tokens: rows of the token buffers */
     int max_q;            /* tokens of the longest sequence; picks the kernel, the result does not depend on it */
@@ -90,9 +91,14 @@ size_t fiber_attn_paged_workspace(const fiber_kv_view_t *kv, const fiber_ragged_
  * scores, softmax and sums in fp32, probabilities and the output rounded to the cache's
  * type. d_q and d_out: rows of n_heads * head_dim values, ldq / ldo elements apart (16-byte
  * aligned, the cache's type). Cache positions that a token does not see do not reach its
- * output, whatever bits they hold. d_ws: workspace, zero-filled before its first use and
- * then reused by any calls of one stream (calls that may overlap need one each). The
- * same call on the same data gives the same bits. */
+ * output, whatever bits they hold.
+ *   At most 128 query heads per KV head. A launch counts its work in 32 bits, so a batch is refused
+ * (FIBER_EARG; fiber_attn_paged_workspace returns 0) from about
+ *     (n_tokens * n_heads / 256 + n_seqs * n_kv_heads) * max_pages * page_size = 1.4e11
+ * on (half of that for groups of 65 to 127 heads), or, where max_q tokens are at most 16 rows per KV
+ * head, (n_tokens * n_heads / 16 + n_seqs * n_kv_heads) * max_pages * page_size = 2.7e11.
+ *   d_ws: workspace, zero-filled before its first use and then reused by any calls of one stream
+ * (calls that may overlap need one each). The same call on the same data gives the same bits. */
 int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t *batch, const void *d_q, int64_t ldq,
                      void *d_out, int64_t ldo, int n_heads, float scale, int window, void *d_ws, size_t ws_bytes,
                      void *stream);

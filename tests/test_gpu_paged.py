@@ -785,3 +785,37 @@ def test_attn_small_weights_of_many_keys_are_not_lost(below, at, group):
     want = small / (1.0 + small)
     tol = 1.05 * U["f16"] * 2 * want + want * (2.0 ** -16 * below + 2.0 ** -15) + 2.0 ** -31 * kv
     assert float((out.double() - want).abs().max()) <= tol
+
+
+# ---- large batches -----------------------------------------------------------------------------
+
+
+def test_attn_131072_tokens_over_their_own_positions():
+    """Eight query heads over one KV head, whose table has room for 2^20 positions."""
+    torch = torch_()
+    n, P, D, H = 131_072, 64, 64, 8
+    g = torch.Generator(device="cuda")
+    g.manual_seed(51)
+    pools = [torch.randn(n // P, 1, P, D, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    table = torch.full(((1 << 20) // P,), -1, dtype=torch.int32, device="cuda")
+    table[:n // P] = torch.randperm(n // P, generator=torch.Generator().manual_seed(1)).int().cuda()
+    q = torch.randn(n, H * D, generator=g, device="cuda").bfloat16()
+    out = torch.zeros_like(q)
+    start = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    view = fb.PagedKV(pools[0].data_ptr(), pools[1].data_ptr(), table.data_ptr(), n_slots=1, max_pages=(1 << 20) // P,
+                      n_pages=n // P, page_size=P, n_kv_heads=1, head_dim=D, dtype=30)
+    batch = fb.RaggedBatch(start.data_ptr(), start.data_ptr() + 4, n_seqs=1, n_tokens=n, max_q=n)
+    ws = torch.zeros(fb.attn_paged_workspace(view, batch, H), dtype=torch.uint8, device="cuda")
+    fb.attn_paged(view, batch, q.data_ptr(), out.data_ptr(), n_heads=H, ldq=H * D, ldo=H * D, scale=0.125, ws=ws.data_ptr(),
+                  ws_bytes=ws.numel())
+    fb.attn_paged_status(ws.data_ptr())
+    k, v = (p[table[:n // P].long()].reshape(-1, D).double() for p in pools)
+    rows = torch.tensor([0, 1, 31, 32, 127, 128, 4095, 65_535, 65_536, 100_000, 131_040, 131_071], device="cuda")
+    seen = torch.arange(n, device="cuda")[None] <= rows[:, None]
+    for h in range(H):
+        x = q[rows, h * D:(h + 1) * D].double()
+        big = float((x.abs() @ k.abs().T).max()) * 0.125
+        p = torch.softmax(torch.where(seen, x @ k.T * 0.125, -math.inf), 1)
+        o, w = p @ v, p @ v.abs()
+        tol = 1.05 * U["bf16"] * (o.abs() + w) + w * (2.0 ** -16 * big + 2.0 ** -15)
+        assert ((out[rows, h * D:(h + 1) * D].double() - o).abs() <= tol).all()

@@ -98,3 +98,20 @@ def test_null_structs_and_empty_batches():
     assert L.fiber_attn_paged(None, None, None, 0, None, 0, 0, C.c_float(1.0), 0, None, 0, None) == -1
     with pytest.raises(fb.FiberError):
         fb.attn_paged_workspace(view(head_dim=96), batch(), 4)
+
+
+@pytest.mark.parametrize("positions,tokens,seqs,max_q", [
+    (131_072, 131_072, 1, 131_072), (1 << 20, 16_384, 32, 512), (1 << 20, 131_072, 1, 131_072), (1 << 20, 4096, 4096, 1)])
+def test_large_batches_that_the_count_has_room_for_are_taken(positions, tokens, seqs, max_q):
+    """Of 64 query and 8 KV heads."""
+    kv = view(page_size=64, max_pages=positions // 64, n_kv_heads=8)
+    assert fb.attn_paged_workspace(kv, batch(n_seqs=seqs, n_tokens=tokens, max_q=max_q), 64) > 0
+
+
+@pytest.mark.parametrize("positions,tokens,heads,kv_heads", [
+    (1 << 24, 1 << 20, 64, 8), (1 << 20, 1 << 20, 64, 8), (16, 1 << 24, 128, 1), (64, 2 ** 31 - 1, 1, 1)])
+def test_larger_ones_are_refused(positions, tokens, heads, kv_heads):
+    kv = view(page_size=16, max_pages=positions // 16, n_kv_heads=kv_heads)
+    for max_q in (1, tokens):
+        with pytest.raises(fb.FiberError, match="too large"):
+            fb.attn_paged_workspace(kv, batch(n_tokens=tokens, max_q=max_q), heads)
