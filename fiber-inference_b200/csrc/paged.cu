@@ -380,5 +380,7 @@ extern "C" int fiber_attn_paged_status(const void *d_ws, void *stream) {
     cudaError_t e = cudaMemcpyAsync(&status, d_ws, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
     if (e != cudaSuccess) return fail(FIBER_ECUDA, "fiber_attn_paged_status: %s", cudaGetErrorString(e));
+    if (status == PG_BAD_BATCH) return fail(FIBER_EARG, "fiber_attn_paged: q_start decreases");
+    if (status == PG_BAD_SM) return fail(FIBER_ECUDA, "fiber_attn_paged: shared or tensor memory is not where the kernel needs it");
     return status == 0 ? FIBER_OK : fail(FIBER_ETIMEOUT, "fiber_attn_paged: a wait inside the kernel gave up");
 }

@@ -203,11 +203,13 @@ struct AttnPagedParams {
     AttnCost cost;
     long long wait_limit;     // cycles after which a wait gives up
     int drill;                // 1: no ring stage is ever free again, so that waits run out; else 0
-    int *status;              // workspace: set to 1 when a wait gave up
+    int *status;              // workspace: PG_GAVE_UP, PG_BAD_SM or PG_BAD_BATCH once that happened
     unsigned int *tickets;    // one per CTA, zero between calls
     float *part_ml;           // [2 * n_cta][rows][2]: running maximum (powers of two) and sum
     float *part_o;            // [2 * n_cta] unnormalised outputs
 };
+
+enum : int { PG_GAVE_UP = 1, PG_BAD_SM = 2, PG_BAD_BATCH = 3 };
 
 constexpr int PG_MAX_SEQS = 128;  // sequences of one launch; larger batches take several
 
@@ -262,15 +264,23 @@ FDEV uint32_t attn_seq_cost(int nq, int kv, const AttnPagedParams &p, int ru, in
     return sum;
 }
 
-// Fill the plan and return T; `longest`: the largest unit's cost, or 0. Up to 32 sequences each warp does it for itself (all write
-// the same), without a barrier: one round trip for the lengths. More are shared among the
-// CTA's threads.
+// Fill the plan and return T; `longest`: the largest unit's cost, or 0. Up to 32 sequences
+// each warp does it for itself (all write the same), without a barrier: one round trip for the
+// lengths. More are shared among the CTA's threads. Where q_start decreases, the sequences may
+// overlap and their costs pass 32 bits: T is 0 then, nothing is done and the status says so.
 template <int THREADS>
 FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, int bk_shift, uint32_t &longest) {
     const int tid = threadIdx.x, lane = tid & 31, ns = p.b.n_seqs;
     constexpr int SHORT = 4;  // sequences of more units are summed by whole warps
+    bool falls = false;
     auto load = [&](int s) {
-        return make_seq(p.b, p.kv, p.b.q_start[s], p.b.q_start[s + 1], p.b.kv_len[s], p.b.slot ? p.b.slot[s] : p.b.slot0 + s);
+        const int start = p.b.q_start[s], end = p.b.q_start[s + 1];
+        falls |= end < start;
+        return make_seq(p.b, p.kv, start, end, p.b.kv_len[s], p.b.slot ? p.b.slot[s] : p.b.slot0 + s);
+    };
+    auto refuse = [&] {
+        if (tid == 0) *p.status = PG_BAD_BATCH;
+        return 0u;
     };
     auto few = [&](const SeqInfo &q, int nu) {
         uint32_t sum = 0;
@@ -288,6 +298,8 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
     if (ns <= 32) {
         SeqInfo q = {0, 0, 0, 0};
         if (lane < ns) q = load(lane);
+        longest = 0;
+        if (__any_sync(0xffffffffu, falls)) return refuse();
         const int nu = fdiv(q.nq * p.group + ru - 1, p.by_ru);
         uint32_t sum = nu <= SHORT ? few(q, nu) : 0;
         for (unsigned big = __ballot_sync(0xffffffffu, nu > SHORT); big; big &= big - 1) {
@@ -313,7 +325,7 @@ FDEV uint32_t attn_plan_build(AttnPlan &pl, const AttnPagedParams &p, int ru, in
         pl.prefix[s + 1] = nu <= SHORT ? few(q, nu) : 0;
     }
     if (tid == 0) pl.prefix[0] = 0;
-    __syncthreads();
+    if (__syncthreads_or(falls)) return refuse();
     for (int s = tid >> 5; s < ns; s += THREADS / 32) {
         const int4 q = pl.seq[s];
         if (fdiv(q.y * p.group + ru - 1, p.by_ru) <= SHORT) continue;

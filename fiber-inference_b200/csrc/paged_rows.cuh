@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         if (lane == 0)
             for (uint32_t s = 0; s < NST && s < it; s++)
                 pg_drain(&sh.full[s], (s + (it - 1 - s) / NST * NST) / NST & 1);
-        if (lane == 0 && sh.fail) *p.status = 1;
+        if (lane == 0 && sh.fail) *p.status = PG_GAVE_UP;
         return;
     }
 
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(PR_THREADS, PR_CTAS_PER_SM) attn_rows_kernel(c
         if (u.u0 + u.cost >= x1) break;
         attn_unit_next(u, sh.plan, p, PR_ROWS, PR_BK_SHIFT);
     }
-    if (lane == 0 && sh.fail) *p.status = 1;
+    if (lane == 0 && sh.fail) *p.status = PG_GAVE_UP;
     pr_bar();
     if (sh.bad && !sh.fail) attn_exact_rows<HD, BF>(p, sh.plan, n_cta, sh.joined, PR_ROWS, PR_BK_SHIFT, PR_WARPS);
 }

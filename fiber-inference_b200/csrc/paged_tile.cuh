@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
     PtShared &sh = *reinterpret_cast<PtShared *>(ring + NST * TB);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (pg_saddr(pt_raw) & 1023u) {  // never: the operand tiles must start on 1024 bytes
-        if (tid == 0) *p.status = 2;
+        if (tid == 0) *p.status = PG_BAD_SM;
         return;
     }
     if (tid == 0) {
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
     uint32_t longest;
     const uint32_t total = attn_plan_build<PT_THREADS>(sh.plan, p, ru, PT_BK_SHIFT, longest);
     constexpr uint32_t tmem = 0;  // all 512 columns
-    if (sh.tmem != tmem && tid == 0) *p.status = 2;
+    if (sh.tmem != tmem && tid == 0) *p.status = PG_BAD_SM;
     const int n_cta = attn_ctas(p, total, longest), cta = blockIdx.x;
     if (tid == 0) sh.n_cta = n_cta;
 
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_tile_kernel(const __grid_c
     }
     pt_fence_before();
     __syncthreads();
-    if (tid == 0 && sh.fail) *p.status = 1;
+    if (tid == 0 && sh.fail) *p.status = PG_GAVE_UP;
     if (warp == 8) {
         pt_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem) : "memory");

@@ -114,7 +114,7 @@ def attn_paged(kv: PagedKV, batch: RaggedBatch, q: int, out: int, *, n_heads: in
 
 
 def attn_paged_status(ws: int, stream=None):
-    """Waits for the stream; raises if a bounded wait inside an attn_paged call gave up."""
+    """Waits for the stream; raises if a bounded wait inside an attn_paged call gave up, or q_start decreased."""
     _check(_paged_lib().fiber_attn_paged_status(ws, _stream_ptr(stream)), "fiber_attn_paged_status")
 
 

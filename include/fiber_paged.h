@@ -103,8 +103,9 @@ int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t *batch, con
                      void *d_out, int64_t ldo, int n_heads, float scale, int window, void *d_ws, size_t ws_bytes,
                      void *stream);
 
-/* Waits for `stream` and reports whether a bounded wait inside a fiber_attn_paged call on
- * this workspace gave up (FIBER_ETIMEOUT; zero-fill the workspace before using it again). */
+/* Waits for `stream` and reports whether a bounded wait inside a fiber_attn_paged call on this
+ * workspace gave up (FIBER_ETIMEOUT), or a call found a decreasing q_start and wrote nothing for its
+ * sequences (FIBER_EARG). Zero-fill the workspace before using it again. */
 int fiber_attn_paged_status(const void *d_ws, void *stream);
 
 /* Drill, for a program to try out how it takes a call whose waits give up: while `on`, the kernels of

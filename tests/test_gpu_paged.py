@@ -819,3 +819,28 @@ def test_attn_131072_tokens_over_their_own_positions():
         o, w = p @ v, p @ v.abs()
         tol = 1.05 * U["bf16"] * (o.abs() + w) + w * (2.0 ** -16 * big + 2.0 ** -15)
         assert ((out[rows, h * D:(h + 1) * D].double() - o).abs() <= tol).all()
+
+
+# ---- sequences that overlap ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n_seqs", [3, 40, 140])
+@pytest.mark.parametrize("nq", [2, 30], ids=["rows", "tile"])
+def test_attn_decreasing_q_start_is_reported_and_nothing_is_written(nq, n_seqs):
+    torch = torch_()
+    s = Setup([(nq, 50)] * n_seqs, 2, 1, 64, "f16", 16, seed=61)
+    s.attend()
+    s.check()
+    good = s.out.clone()
+    start = s.dstart.clone()
+    s.dstart[2] = 1
+    s.out.fill_(7.0)
+    s.attend()
+    with pytest.raises(fb.FiberError, match="q_start decreases"):
+        fb.attn_paged_status(s.ws.data_ptr())
+    last = s.starts[128] if n_seqs > 128 else s.n  # a launch takes 128 sequences
+    assert (s.out[:last] == 7.0).all() and torch.equal(s.out[last:], good[last:])
+    s.ws.zero_()
+    s.dstart.copy_(start)
+    s.attend()
+    s.check()
