@@ -276,6 +276,8 @@ extern "C" int fiber_kv_append(const fiber_kv_view_t *kv, const fiber_ragged_t *
     if (rope && (!rope->table || !aligned16(rope->table) || rope->max_pos <= 0 || rope->dim <= 0 || rope->dim % 16 ||
                  rope->dim > hd))
         return fail(FIBER_EARG, "%s: bad rope (dim %d, a multiple of 16 up to head_dim; table 16-byte aligned)", fn, rope->dim);
+    if (d_q && d_q == d_q_out && (in_type == FIBER_TYPE_F32 || ldq != ldo))
+        return fail(FIBER_EARG, "%s: in place, q and q_out have one type and one row stride", fn);
     AppendParams p;
     memset(&p, 0, sizeof(p));
     p.kv = dev_view(kv);
@@ -325,6 +327,8 @@ extern "C" int fiber_attn_paged(const fiber_kv_view_t *kv, const fiber_ragged_t 
     if (!d_ws || !aligned16(d_ws) || ws_bytes < ws_bytes_of(shape, hd))
         return fail(FIBER_EARG, "%s: workspace of %zu bytes, 16-byte aligned, needed (%zu given)", fn,
                     ws_bytes_of(shape, hd), ws_bytes);
+    if (d_q == d_out)  // a row that is computed again reads its query after its first result is stored
+        return fail(FIBER_EARG, "%s: d_q and d_out are the same buffer", fn);
     AttnPagedParams p;
     memset(&p, 0, sizeof(p));
     p.kv = dev_view(kv);

@@ -74,8 +74,9 @@ typedef struct {
  * type), heads contiguous, token rows ldq / ldk / ldv elements apart, so the parts of one
  * fused q|k|v row can be passed. Keys are rotated and rounded once into k_pool, values
  * rounded into v_pool, queries rotated into d_q_out (rows of ldo elements, the cache's
- * type; may be d_q when the types agree). d_q and d_q_out null: keys and values only.
- * rope null: no rotation. Rows of all buffers are 16-byte aligned. */
+ * type; may be d_q when types and row strides agree, and overlaps no other input). d_q and
+ * d_q_out null: keys and values only. rope null: no rotation. Rows of all buffers are 16-byte
+ * aligned. */
 int fiber_kv_append(const fiber_kv_view_t *kv, const fiber_ragged_t *batch, int in_type, const void *d_q,
                     int64_t ldq, const void *d_k, int64_t ldk, const void *d_v, int64_t ldv, int n_heads,
                     const fiber_rope_t *rope, void *d_q_out, int64_t ldo, void *stream);
@@ -90,7 +91,7 @@ size_t fiber_attn_paged_workspace(const fiber_kv_view_t *kv, const fiber_ragged_
  *     out = sum_j softmax_j(scale * q . k_j) v_j,
  * scores, softmax and sums in fp32, probabilities and the output rounded to the cache's
  * type. d_q and d_out: rows of n_heads * head_dim values, ldq / ldo elements apart (16-byte
- * aligned, the cache's type). Cache positions that a token does not see do not reach its
+ * aligned, the cache's type), that do not overlap. Cache positions that a token does not see do not reach its
  * output, whatever bits they hold.
  *   At most 128 query heads per KV head. A launch counts its work in 32 bits, so a batch is refused
  * (FIBER_EARG; fiber_attn_paged_workspace returns 0) from about

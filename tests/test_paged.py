@@ -115,3 +115,14 @@ def test_larger_ones_are_refused(positions, tokens, heads, kv_heads):
     for max_q in (1, tokens):
         with pytest.raises(fb.FiberError, match="too large"):
             fb.attn_paged_workspace(kv, batch(n_tokens=tokens, max_q=max_q), heads)
+
+
+def test_attn_refuses_its_output_over_its_queries():
+    with pytest.raises(fb.FiberError, match="same buffer"):
+        attend(q=A, out=A)
+
+
+@pytest.mark.parametrize("bad", [dict(in_type=0, ld_out=512), dict(in_type=1, ld_out=256), dict(in_type=1, ld_out=1024)])
+def test_append_in_place_takes_one_type_and_one_stride(bad):
+    with pytest.raises(fb.FiberError, match="in place"):
+        append(**bad)
