@@ -64,7 +64,8 @@ int check_view(const char *fn, const fiber_kv_view_t *kv) {
     if (kv->n_kv_heads <= 0 || kv->n_pages <= 0 || kv->n_slots <= 0 || kv->max_pages <= 0)
         return fail(FIBER_EARG, "%s: bad cache shape (kv_heads=%d pages=%d slots=%d max_pages=%d)", fn, kv->n_kv_heads,
                     kv->n_pages, kv->n_slots, kv->max_pages);
-    if ((int64_t)kv->max_pages * P > 0x7fffffff) return fail(FIBER_EARG, "%s: a slot holds more than 2^31 - 1 positions", fn);
+    // positions are rounded up to whole tiles and pages in 32 bits
+    if ((int64_t)kv->max_pages * P > 0x7fffff00) return fail(FIBER_EARG, "%s: a slot holds more than 2^31 - 256 positions", fn);
     if (!aligned16(kv->k_pool) || !aligned16(kv->v_pool)) return fail(FIBER_EARG, "%s: pools must be 16-byte aligned", fn);
     if (!stride_ok(kv->pos_stride, kv->head_dim) || !stride_ok(kv->head_stride, kv->head_dim) ||
         !stride_ok(kv->page_stride, kv->head_dim))

@@ -37,7 +37,7 @@ typedef struct {
     int n_kv_heads;
     int page_size; /* 16, 32, 64, 128 or 256 positions */
     int n_pages;   /* pages in each pool */
-    int n_slots, max_pages; /* page_table is [n_slots][max_pages] */
+    int n_slots, max_pages; /* page_table is [n_slots][max_pages]; max_pages * page_size <= 2^31 - 256 */
     int64_t page_stride, head_stride, pos_stride;
     void *k_pool, *v_pool;     /* device */
     const int32_t *page_table; /* device */

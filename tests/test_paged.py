@@ -126,3 +126,10 @@ def test_attn_refuses_its_output_over_its_queries():
 def test_append_in_place_takes_one_type_and_one_stride(bad):
     with pytest.raises(fb.FiberError, match="in place"):
         append(**bad)
+
+
+def test_slots_of_almost_2_to_the_31_positions():
+    for f in (attend, append):
+        with pytest.raises(fb.FiberError, match="2\\^31"):
+            f(kv=view(page_size=16, max_pages=(1 << 27) - 15, n_kv_heads=1))
+    assert fb.attn_paged_workspace(view(page_size=16, max_pages=(1 << 27) - 16, n_kv_heads=1), batch(), 4) > 0
