@@ -844,3 +844,24 @@ def test_attn_decreasing_q_start_is_reported_and_nothing_is_written(nq, n_seqs):
     s.dstart.copy_(start)
     s.attend()
     s.check()
+
+
+# ---- many sequences in the tile kernel ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("dim,dtype,n_seqs", [(64, "f16", 40), (128, "bf16", 40), (64, "bf16", 150), (128, "f16", 150)])
+def test_attn_chunks_of_many_sequences(n_seqs, dim, dtype, window):
+    """More sequences than a warp has lanes, and than a launch takes: chunks, single tokens and absences, a few
+    sequences of many units."""
+    rng = np.random.default_rng(n_seqs + window)
+    lens = []
+    for i in range(n_seqs):
+        n = int(rng.choice([0, 1, 1, 5, 17, 40]))
+        lens.append((n, n + int(rng.integers(0, 120))))
+    lens[3], lens[n_seqs - 2] = (300, 420), (0, 0)
+    s = Setup(lens, 6, 2, dim, dtype, 16, window=window, seed=n_seqs)
+    for _ in range(2):  # the launches of a call share the workspace
+        s.out.fill_(7.0)
+        s.attend()
+    s.check()

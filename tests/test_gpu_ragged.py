@@ -146,3 +146,57 @@ def test_a_pass_whose_waits_give_up_says_so_and_the_next_one_is_right(tiny_model
         am2, lg2 = step()
         assert np.array_equal(am2, am) and np.array_equal(lg2, lg)
     assert ctx.prefill(kv, prompt, slot=0) == greedy
+
+
+def _tp_worker(rank, world, nid, path, seqs, cuts, q):
+    try:
+        ctx = fb.Context(fb.HostModel(path), device=rank, max_seq=256, tp=(rank, world, nid), max_batch=3)
+        kv = ctx.kv(256, max_batch=3)
+        out, done = [], [0] * len(seqs)
+        for cut in cuts:
+            which = [i for i in range(len(seqs)) if cut[i] > done[i]]
+            am, lg = ctx.forward_ragged(kv, which, [done[i] for i in which], [seqs[i][done[i]:cut[i]] for i in which])
+            out.append((am, lg))
+            done = list(cut)
+        q.put((rank, out, None))
+        ctx.close()
+    except Exception as e:  # report instead of hanging the parent
+        q.put((rank, None, repr(e)))
+
+
+def test_two_ranks_match_the_oracle(tiny_model):
+    import torch
+    import torch.multiprocessing as mp
+
+    if not torch.cuda.is_available() or torch.cuda.device_count() < 2:
+        pytest.skip("needs 2 GPUs")
+    path = tiny_model("tp")
+    rng = np.random.default_rng(6)
+    seqs = [rng.integers(1, fb.HostModel(path).params.vocab_size, n).astype(np.int32) for n in (60, 1, 33)]
+    cuts = [[40, 1, 30], [41, 1, 33], [60, 1, 33]]
+    nid = fb.tp_unique_id()
+    c = mp.get_context("spawn")
+    q = c.Queue()
+    procs = [c.Process(target=_tp_worker, args=(r, 2, nid, path, seqs, cuts, q)) for r in range(2)]
+    for pr in procs:
+        pr.start()
+    res = {}
+    try:
+        for _ in procs:
+            rank, out, err = q.get(timeout=300)
+            res[rank] = (out, err)
+    finally:
+        for pr in procs:
+            pr.join(timeout=60)
+            if pr.is_alive():
+                pr.kill()
+    done = [0] * len(seqs)
+    for step, cut in enumerate(cuts):
+        which = [i for i in range(len(seqs)) if cut[i] > done[i]]
+        want = {i: _oracle_logits(path, seqs[i][:cut[i]]) for i in which}
+        for rank in range(2):
+            out, err = res[rank]
+            assert err is None, err
+            for k, i in enumerate(which):
+                _check(*out[step], k, want[i])
+        done = list(cut)
