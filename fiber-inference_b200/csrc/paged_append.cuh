@@ -7,8 +7,9 @@
 // cache), rounded once to the cache's type.
 //
 // Bound by bytes: every value is read and written once, 3 operations each. 17,055 tokens
-// of 32 + 8 + 8 heads of 128 (bf16, 420 MB) take 75 us, 5.6 TB/s or 85% of a plain copy's
-// rate; one token takes 2.8 us on the device, the latency of two dependent lookups.
+// of 32 + 8 + 8 heads of 128 (bf16, 420 MB) take 74 us, 5.7 TB/s or 87% of a plain copy's
+// rate; one token takes 2.8 us on the device, the latency of two dependent lookups, and 512
+// tokens of 32 + 4 + 4 heads of 64 (fp32 in, 8 MB) 3.8 us.
 #pragma once
 #include "paged.cuh"
 

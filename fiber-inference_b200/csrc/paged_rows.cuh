@@ -8,9 +8,9 @@
 // its own (m, l, o), so no barrier is needed per tile; the four states are joined at the
 // end of a unit. mma.sync m16n8k16 serves here because a 16-row operand fills it, where a
 // 128-row tcgen05 tile would be seven eighths empty: the tile kernel streams such rows at
-// 4.4 TB/s, this one at 5.7 to 6.2 (two tokens over 242,802 positions, 995 MB: 161 us, 94% of
+// 4.4 to 4.8 TB/s, this one at 5.7 to 6.2 (two tokens over 242,802 positions, 995 MB: 161 us, 94% of
 // a plain copy's rate; 64 tokens over 211,722 positions in pages of 16: 144 us, 92%). A short
-// call is latency: one token over 384 positions takes 6.8 us on the device, of which 4.9 remain
+// call is latency: one token over 384 positions takes 7.0 us on the device, of which 4.9 remain
 // at 101 positions.
 #pragma once
 #include "paged.cuh"
